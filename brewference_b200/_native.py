@@ -71,6 +71,21 @@ class ModelWeights(ctypes.Structure):
                                       "q_bias", "k_bias", "v_bias")]
 
 
+class KvConfig(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("n_layers", "n_heads", "n_kv_heads", "head_size", "max_seqs", "max_tokens",
+                                              "page_tokens", "n_pages")]
+
+
+class KvRowsC(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("seq", "pos", "row_start")] + \
+               [(n, ctypes.c_int32) for n in ("n_seqs", "n_rows", "max_rows")]
+
+
+class KvRopeC(ctypes.Structure):
+    _fields_ = [("mode", ctypes.c_int32), ("base", ctypes.c_double), ("scale", ctypes.c_double),
+                ("qnorm", ctypes.c_void_p), ("knorm", ctypes.c_void_p), ("eps", ctypes.c_double)]
+
+
 def lib():
     global _lib
     if _lib is not None:
@@ -130,6 +145,19 @@ def lib():
                                       ctypes.POINTER(I64)]),
         "brew_model_load_gguf": (I, [ctypes.c_char_p, ctypes.c_int32, c_void_pp]),
         "brew_selftest_wait_timeout": (I, [I64, c_i32p]),
+        "brew_kv_create": (I, [ctypes.POINTER(KvConfig), c_void_pp]),
+        "brew_kv_free": (I, [V]),
+        "brew_kv_info": (I, [V, ctypes.POINTER(I64), c_i32p]),
+        "brew_kv_reserve": (I, [V, ctypes.c_int32, ctypes.c_int32, V]),
+        "brew_kv_release": (I, [V, ctypes.c_int32, V]),
+        "brew_kv_check": (I, [V]),
+        "brew_kv_append_dev": (I, [V, ctypes.c_int32, V, V, I64, V, V, I64, ctypes.POINTER(KvRowsC),
+                                   ctypes.POINTER(KvRopeC), V]),
+        "brew_kv_read_dev": (I, [V, ctypes.c_int32, V, V, I64, ctypes.POINTER(KvRowsC), V]),
+        "brew_kv_workspace_bytes": (I64, [V]),
+        "brew_kv_attend_dev": (I, [V, ctypes.c_int32, V, I64, V, I64, ctypes.POINTER(KvRowsC), ctypes.c_int32,
+                                   ctypes.c_float, V, V]),
+        "brew_logprobs_dev": (I, [V, I64, ctypes.c_int32, ctypes.c_int32, V, V, V, ctypes.c_int32, V, V, V]),
         "brew_prep_bytes": (I64, [ctypes.c_int32, ctypes.c_int32]),
         "brew_prepare_input_dev": (I, [V, ctypes.c_int32, ctypes.c_int32, V, V]),
         "brew_matmul_prepared_dev": (I, [V, V, V, I64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, V]),

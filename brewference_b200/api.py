@@ -164,6 +164,111 @@ class GemmPlan:
             pass
 
 
+ROPE_NONE, ROPE_HALF, ROPE_INTERLEAVED = 0, 1, 2   # KvRope modes
+MAX_TOP = 32                                       # alternatives of Logits.logprobs_device
+
+
+class KvRows:
+    """The rows of a KvCache call (brew_kv_rows): device addresses of int32
+    arrays.  Entry i holds rows row_start[i] .. row_start[i + 1] - 1, at
+    positions pos[i], pos[i] + 1, ... of sequence seq[i]; without row_start,
+    row i.  Built once, it can be passed to any number of calls (the arrays
+    are read on the device, when each call runs)."""
+
+    def __init__(self, seq_ptr: int, pos_ptr: int, n_seqs: int, n_rows: int = None, max_rows: int = 1,
+                 row_start_ptr: int = 0):
+        self.c = N.KvRowsC(seq_ptr or None, pos_ptr or None, row_start_ptr or None, n_seqs,
+                           n_seqs if n_rows is None else n_rows, max_rows)
+        self.ref = ctypes.byref(self.c)
+
+
+class KvRope:
+    """Head-wise RMSNorm (device weights, 0: none) and position rotation of q
+    and k in KvCache.append (brew_kv_rope)."""
+
+    def __init__(self, mode: int, base: float = 1e4, scale: float = 1.0, qnorm_ptr: int = 0, knorm_ptr: int = 0,
+                 eps: float = 1e-6):
+        self.c = N.KvRopeC(mode, base, scale, qnorm_ptr or None, knorm_ptr or None, eps)
+        self.ref = ctypes.byref(self.c)
+
+
+class KvCache:
+    """A paged K/V cache in 4 bits (brew_kv_*): blocks of 32 values with one
+    fp16 scale, 0.5625 bytes a value.  Device pointers are addresses; strides
+    are in floats."""
+
+    def __init__(self, n_layers: int, n_heads: int, n_kv_heads: int, head_size: int, max_seqs: int, max_tokens: int,
+                 page_tokens: int = 64, n_pages: int = 0):
+        self.handle = None
+        c = N.KvConfig(n_layers, n_heads, n_kv_heads, head_size, max_seqs, max_tokens, page_tokens, n_pages)
+        h = ctypes.c_void_p()
+        N.check(N.lib().brew_kv_create(ctypes.byref(c), ctypes.byref(h)), "kv_create")
+        self.handle = h.value
+
+    def info(self):
+        """(bytes of all pages, free pages)"""
+        b, f = ctypes.c_int64(), ctypes.c_int32()
+        N.check(N.lib().brew_kv_info(self.handle, ctypes.byref(b), ctypes.byref(f)), "kv_info")
+        return b.value, f.value
+
+    def reserve(self, seq: int, n_tokens: int, stream: int = 0) -> None:
+        """Pages for positions 0 .. n_tokens - 1 of a sequence."""
+        N.check(N.lib().brew_kv_reserve(self.handle, seq, n_tokens, stream or None), "kv_reserve")
+
+    def release(self, seq: int, stream: int = 0) -> None:
+        N.check(N.lib().brew_kv_release(self.handle, seq, stream or None), "kv_release")
+
+    def append(self, layer: int, q_out_ptr: int, q_ptr: int, ldq: int, k_ptr: int, v_ptr: int, ldkv: int, rows: KvRows,
+               rope: KvRope = None, stream: int = 0) -> None:
+        """Norm and rotation of q (into q_out) and k, and k and v into the
+        cache; q_ptr and q_out_ptr 0: k and v only."""
+        N.check(N.lib().brew_kv_append_dev(self.handle, layer, q_out_ptr or None, q_ptr or None, ldq, k_ptr, v_ptr, ldkv,
+                                           rows.ref, rope.ref if rope is not None else None, stream or None), "kv_append")
+
+    def read(self, layer: int, k_out_ptr: int, v_out_ptr: int, ld: int, rows: KvRows, stream: int = 0) -> None:
+        """The values that the rows' stored k and v stand for."""
+        N.check(N.lib().brew_kv_read_dev(self.handle, layer, k_out_ptr or None, v_out_ptr or None, ld, rows.ref,
+                                         stream or None), "kv_read")
+
+    def workspace_bytes(self) -> int:
+        """Device bytes of attend's workspace, zero-filled before its first use."""
+        return int(N.lib().brew_kv_workspace_bytes(self.handle))
+
+    def attend(self, layer: int, out_ptr: int, ldo: int, q_ptr: int, ldq: int, rows: KvRows, window: int,
+               workspace_ptr: int, scale: float = 0.0, stream: int = 0) -> None:
+        """Causal attention of the rows over their sequences' positions (the
+        last `window` of them when > 0); scale 0: 1 / sqrt(head_size)."""
+        N.check(N.lib().brew_kv_attend_dev(self.handle, layer, out_ptr, ldo, q_ptr, ldq, rows.ref, window, scale,
+                                           workspace_ptr, stream or None), "kv_attend")
+
+    def check(self) -> None:
+        """Synchronises; raises if a call since the last check skipped a row."""
+        N.check(N.lib().brew_kv_check(self.handle), "kv_check")
+
+    def free(self):
+        if self.handle:
+            N.lib().brew_kv_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class Logits:
+    """Scores of given tokens under rows of logits (brew_logprobs_dev)."""
+
+    @staticmethod
+    def logprobs_device(logits_ptr: int, ld: int, vocab: int, rows: int, tokens_ptr: int, logprob_ptr: int,
+                        entropy_ptr: int = 0, top: int = 0, top_ids_ptr: int = 0, top_logprobs_ptr: int = 0,
+                        stream: int = 0) -> None:
+        N.check(N.lib().brew_logprobs_dev(logits_ptr, ld, vocab, rows, tokens_ptr or None, logprob_ptr or None,
+                                          entropy_ptr or None, top, top_ids_ptr or None, top_logprobs_ptr or None,
+                                          stream or None), "logprobs")
+
+
 def tp_rows(rows: int, nranks: int, rank: int):
     """Rows [r0, r1) of an N-row matrix that `rank` of `nranks` owns in the
     tensor-parallel forward."""

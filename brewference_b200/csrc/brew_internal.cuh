@@ -39,6 +39,20 @@ Context& ctx();
 std::mutex& api_mutex();
 int ensure_init();
 
+// Makes the library's device current for one call and the caller's again
+// after it.
+struct DeviceScope {
+    int before = -1;
+    int rc;
+    DeviceScope() {
+        if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+        rc = ensure_init();
+    }
+    ~DeviceScope() {
+        if (before >= 0 && ctx().initialized && before != ctx().device) cudaSetDevice(before);
+    }
+};
+
 int run_matvec(brew_tensor t, int64_t weights_offset, const float* x_dev, int K, int N, float* y_dev, int batch,
                cudaStream_t stream);
 int run_matvec_prepared(brew_tensor t, int64_t weights_offset, const uint8_t* prep, int K, int N, float* y, int batch,

@@ -1,0 +1,552 @@
+// kv.cu — the paged 4-bit K/V cache: its handle (pages, reservations), the
+// append and read kernels and the C ABI of both and of the attention.
+#include <cmath>
+#include <new>
+#include <vector>
+
+#include "brew_internal.cuh"
+#include "kv.cuh"
+
+struct brew_kv_s {
+    brew_kv_config c = {};
+    int max_pages = 0;              // pages of one sequence
+    int page_shift = 0;
+    int64_t layer_bytes = 0;
+    uint8_t* pool = nullptr;
+    int32_t* table = nullptr;       // [max_seqs][max_pages]
+    int32_t* reserved = nullptr;    // [max_seqs]
+    unsigned int* err = nullptr;
+    int device = 0;
+    std::mutex mu;
+    std::vector<int32_t> free_pages;             // the last one is handed out next
+    std::vector<std::vector<int32_t>> seq_pages;
+};
+
+namespace brew {
+namespace {
+
+// Page ids of positions first .. first + n - 1 pages of a sequence, and then
+// its reserved positions: launch parameters, so that the call stays
+// asynchronous and needs no staging buffer.
+struct KvIds {
+    int32_t id[120];
+};
+
+__global__ void kv_table_kernel(int32_t* row, int first, int n, KvIds ids, int32_t* reserved, int tokens) {
+    if ((int)threadIdx.x < n) row[first + threadIdx.x] = ids.id[threadIdx.x];
+    if (threadIdx.x == 0) *reserved = tokens;
+}
+
+int set_pages(brew_kv_s* kv, int seq, size_t first, size_t end, int tokens, cudaStream_t s) {
+    const std::vector<int32_t>& pages = kv->seq_pages[seq];
+    int32_t* row = kv->table + (int64_t)seq * kv->max_pages;
+    do {
+        KvIds ids;
+        const int n = (int)std::min<size_t>(end - first, 120);
+        for (int i = 0; i < n; ++i) ids.id[i] = pages[first + i];
+        const int now = (size_t)n == end - first ? tokens : (int)((first + n) << kv->page_shift);
+        kv_table_kernel<<<1, 128, 0, s>>>(row, (int)first, n, ids, kv->reserved + seq, now);
+        BREW_CUDA(cudaGetLastError());
+        count_launch();
+        first += n;
+    } while (first < end);
+    return BREW_OK;
+}
+
+// ---- append -------------------------------------------------------------
+// One CTA per row.  The row's angles are computed once, in 64 bits (a
+// position of 10^5 leaves 32 bits no digit of the angle), and shared by all
+// heads; norm and rotation run in 64 bits too and are rounded once, because
+// the 4-bit code of a value next to a rounding border depends on its last
+// bit.  A vector (one head of q, k or v) is held by LPV lanes, 4 dims each
+// (twice for heads of 256); a block of 32 values is 8 lanes.
+constexpr int AP_THREADS = 256;
+
+template <int R>
+__global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(const __grid_constant__ KvAppendParams p) {
+    constexpr int HD = 32 * R;
+    constexpr int LPV = R == 1 ? 8 : R == 2 ? 16 : 32;   // lanes a vector (R = 3: 24 of them hold values)
+    constexpr int NV = R == 8 ? 2 : 1;                   // float4s a lane
+    constexpr int VPW = 32 / LPV;                        // vectors of a warp
+    __shared__ double cs[HD / 2], sn[HD / 2];
+    const KvEntry e = kv_entry(p.kv, p.rows, blockIdx.y, threadIdx.x == 0 && blockIdx.x == 0);
+    const int j = blockIdx.x;
+    if (j >= e.rows) return;
+    const int pos = e.pos0 + j;
+    const int64_t row = e.row0 + j;
+    if (p.rope != BREW_KV_ROPE_NONE) {
+        for (int i = threadIdx.x; i < HD / 2; i += AP_THREADS) {
+            const double a = (double)pos * p.rope_scale * exp2(-2.0 * i * p.log2_base_hd);
+            sincos(a, &sn[i], &cs[i]);
+        }
+        __syncthreads();
+    }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int l = lane % LPV;
+    const bool act = R != 3 || l < 24;
+    const int hq = p.q ? p.kv.n_heads : 0, hk = p.kv.n_kv;
+    const int nvec = hq + 2 * hk;
+    for (int v0 = warp * VPW; v0 < nvec; v0 += AP_THREADS / 32 * VPW) {   // uniform over the warp
+        const int v = v0 + lane / LPV;
+        const bool on = act && v < nvec;
+        const bool isq = v < hq, isk = !isq && v < hq + hk;
+        const int head = isq ? v : isk ? v - hq : v - hq - hk;
+        const float* src = (isq ? p.q + row * p.ldq : (isk ? p.k : p.v) + row * p.ldkv) + (int64_t)head * HD;
+        const float* w = isq ? p.qnorm : isk ? p.knorm : nullptr;
+        float x[NV][4];
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const float4 t = on ? *reinterpret_cast<const float4*>(src + 128 * n + 4 * l) : make_float4(0, 0, 0, 0);
+            x[n][0] = t.x; x[n][1] = t.y; x[n][2] = t.z; x[n][3] = t.w;
+        }
+        double inv = 1.0;
+        if (p.qnorm || p.knorm) {   // uniform
+            double ss = 0.0;
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) ss += (double)x[n][c] * (double)x[n][c];
+#pragma unroll
+            for (int o = LPV / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            inv = 1.0 / sqrt(ss / HD + p.eps);
+        }
+        float y[NV][4];
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) y[n][c] = x[n][c];
+        if (on && (isq || isk) && (w || p.rope != BREW_KV_ROPE_NONE)) {
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                const int d0 = 128 * n + 4 * l;
+                double a[4], b[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) a[c] = w ? (double)x[n][c] * inv * (double)w[d0 + c] : (double)x[n][c];
+                if (p.rope == BREW_KV_ROPE_HALF) {   // pairs (d, d + hd / 2)
+                    const bool lowd = d0 < HD / 2;
+                    const int m0 = lowd ? d0 + HD / 2 : d0 - HD / 2;
+                    const float4 t = *reinterpret_cast<const float4*>(src + m0);
+                    b[0] = t.x; b[1] = t.y; b[2] = t.z; b[3] = t.w;
+                    if (w)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) b[c] = b[c] * inv * (double)w[m0 + c];
+                    const int i0 = lowd ? d0 : m0;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        a[c] = lowd ? a[c] * cs[i0 + c] - b[c] * sn[i0 + c] : b[c] * sn[i0 + c] + a[c] * cs[i0 + c];
+                } else if (p.rope == BREW_KV_ROPE_INTERLEAVED) {   // pairs (2 i, 2 i + 1)
+#pragma unroll
+                    for (int c = 0; c < 4; c += 2) {
+                        const int i = (d0 + c) / 2;
+                        const double r0 = a[c] * cs[i] - a[c + 1] * sn[i], r1 = a[c] * sn[i] + a[c + 1] * cs[i];
+                        a[c] = r0;
+                        a[c + 1] = r1;
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) y[n][c] = (float)a[c];
+            }
+        }
+        __syncwarp();   // q_out may be q: every lane has read before one writes
+        if (on && isq) {
+            float* dst = p.q_out + row * p.ldq + (int64_t)head * HD;
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+                *reinterpret_cast<float4*>(dst + 128 * n + 4 * l) = make_float4(y[n][0], y[n][1], y[n][2], y[n][3]);
+        }
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            // the block's scale: -1/8 of its first value of largest magnitude
+            uint32_t m = 0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) m = max(m, __float_as_uint(y[n][c]) & 0x7fffffffu);
+            uint32_t mb = m;
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+            float mine = y[n][3];
+#pragma unroll
+            for (int c = 2; c >= 0; --c)
+                if ((__float_as_uint(y[n][c]) & 0x7fffffffu) == mb) mine = y[n][c];
+            const uint32_t has = __ballot_sync(0xffffffffu, m == mb) >> (lane & 24) & 255u;
+            const float top = __shfl_sync(0xffffffffu, mine, (lane & 24) + __ffs(has) - 1);
+            float d = top * -0.125f;
+            // fp16 ends at 65504: larger blocks saturate (a NaN stays one)
+            if (fabsf(d) > 65504.0f) d = copysignf(65504.0f, d);
+            const float id = d == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);
+            uint32_t q = 0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int t = (int)truncf(__fadd_rn(__fmul_rn(y[n][c], id), 8.5f));
+                q |= (uint32_t)max(0, min(15, t)) << (4 * c);
+            }
+            const uint32_t next = __shfl_down_sync(0xffffffffu, q, 1);
+            if (!on || isq) continue;
+            uint8_t* grp = kv_group<R>(p.kv, e.seq, pos, head);
+            const int b = 4 * n + l / 8, pg = pos & 15, u = pg >> 3;
+            if (isk) {
+                uint32_t* kq = reinterpret_cast<uint32_t*>(grp);
+                if ((l & 1) == 0) kq[kv_word(R, u, b, (pg & 7) * 4 + (l & 7) / 2)] = q | next << 16;
+            } else {
+                uint16_t* vq = reinterpret_cast<uint16_t*>(grp + 256 * R);
+                vq[2 * kv_word(R, u, b, (l & 7) * 4 + ((pg & 7) >> 1)) + (pg & 1)] = (uint16_t)q;
+            }
+            if ((l & 7) == 0) {
+                uint16_t* sc = reinterpret_cast<uint16_t*>(grp + 512 * R + (isk ? 0 : 32 * R));
+                sc[kv_scale(R, pg, b)] = __half_as_ushort(__float2half_rn(d));
+            }
+        }
+    }
+}
+
+template <int R>
+int append_r(const KvAppendParams& p, cudaStream_t s) {
+    const dim3 grid(p.rows.max_rows, p.rows.n_seqs);
+    kv_append_kernel<R><<<grid, AP_THREADS, 0, s>>>(p);
+    BREW_CUDA(cudaGetLastError());
+    count_launch();
+    return BREW_OK;
+}
+
+// ---- read: the values that stored rows stand for --------------------------
+// One thread per 4 dims of a (row, kv head), k and v both.
+template <int R>
+__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvView kv,
+                                                      const __grid_constant__ KvRowsDev rows, float* k_out,
+                                                      float* v_out, int64_t ld) {
+    const KvEntry e = kv_entry(kv, rows, blockIdx.y, threadIdx.x == 0 && blockIdx.x == 0);
+    const int j = blockIdx.x;
+    if (j >= e.rows) return;
+    const int pos = e.pos0 + j, pg = pos & 15, u = pg >> 3;
+    for (int t = threadIdx.x; t < kv.n_kv * 8 * R; t += 256) {
+        const int hk = t / (8 * R), d4 = t % (8 * R), b = d4 / 8, l = d4 & 7;
+        const uint8_t* grp = kv_group<R>(kv, e.seq, pos, hk);
+        const int64_t o = (e.row0 + j) * ld + (int64_t)hk * 32 * R + 4 * d4;
+        const uint16_t* kq = reinterpret_cast<const uint16_t*>(grp);
+        const uint16_t* sc = reinterpret_cast<const uint16_t*>(grp + 512 * R);
+        const int si = kv_scale(R, pg, b);
+        const uint32_t qk = kq[2 * kv_word(R, u, b, (pg & 7) * 4 + l / 2) + (l & 1)];
+        const uint32_t qv = kq[128 * R + 2 * kv_word(R, u, b, l * 4 + ((pg & 7) >> 1)) + (pg & 1)];
+        const float dk = half_bits_to_float(sc[si]), dv = half_bits_to_float(sc[16 * R + si]);
+        auto val = [](uint32_t q, int c, float d) { return (float)((int)(q >> 4 * c & 15) - 8) * d; };
+        if (k_out)
+            *reinterpret_cast<float4*>(k_out + o) = make_float4(val(qk, 0, dk), val(qk, 1, dk), val(qk, 2, dk), val(qk, 3, dk));
+        if (v_out)
+            *reinterpret_cast<float4*>(v_out + o) = make_float4(val(qv, 0, dv), val(qv, 1, dv), val(qv, 2, dv), val(qv, 3, dv));
+    }
+}
+
+template <int R>
+int read_r(const KvView& kv, const KvRowsDev& rows, float* k, float* v, int64_t ld, cudaStream_t s) {
+    const dim3 grid(rows.max_rows, rows.n_seqs);
+    kv_read_kernel<R><<<grid, 256, 0, s>>>(kv, rows, k, v, ld);
+    BREW_CUDA(cudaGetLastError());
+    count_launch();
+    return BREW_OK;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+int check_rows(const brew_kv_s* kv, int layer, const brew_kv_rows* r) {
+    BREW_CHECK(kv, BREW_ERR_INVALID_ARG, "null K/V cache");
+    BREW_CHECK(r, BREW_ERR_INVALID_ARG, "rows is null");
+    BREW_CHECK(layer >= 0 && layer < kv->c.n_layers, BREW_ERR_INVALID_ARG, "layer %d of %d", layer, kv->c.n_layers);
+    BREW_CHECK(r->n_seqs >= 0 && r->n_seqs <= KV_MAX_SEQS, BREW_ERR_INVALID_ARG, "n_seqs %d (at most %d)", r->n_seqs,
+               KV_MAX_SEQS);
+    BREW_CHECK(r->n_rows >= 0 && r->max_rows >= 0, BREW_ERR_INVALID_ARG, "n_rows %d, max_rows %d", r->n_rows,
+               r->max_rows);
+    if (r->n_seqs == 0) return BREW_OK;
+    BREW_CHECK(r->seq && r->pos, BREW_ERR_INVALID_ARG, "rows: seq and pos must be given");
+    BREW_CHECK(r->row_start || (r->n_rows == r->n_seqs && r->max_rows <= 1), BREW_ERR_INVALID_ARG,
+               "rows without row_start: one row for each sequence (n_rows %d, n_seqs %d, max_rows %d)", r->n_rows,
+               r->n_seqs, r->max_rows);
+    BREW_CHECK(((uintptr_t)r->seq & 3) == 0 && ((uintptr_t)r->pos & 3) == 0 && ((uintptr_t)r->row_start & 3) == 0,
+               BREW_ERR_INVALID_ARG, "rows: unaligned int32 arrays");
+    return BREW_OK;
+}
+
+int check_matrix(const char* what, const void* p, int64_t ld, int64_t width) {
+    BREW_CHECK(p, BREW_ERR_INVALID_ARG, "%s is null", what);
+    BREW_CHECK(aligned16(p) && ld % 4 == 0, BREW_ERR_INVALID_ARG, "%s: rows must start on 16-byte boundaries", what);
+    BREW_CHECK(ld >= width, BREW_ERR_INVALID_ARG, "%s: row stride %lld under its width %lld", what, (long long)ld,
+               (long long)width);
+    return BREW_OK;
+}
+
+KvRowsDev rows_dev(const brew_kv_rows* r) {
+    return {r->seq, r->pos, r->row_start, r->n_seqs, r->n_rows, r->max_rows};
+}
+
+}  // namespace
+
+KvView kv_view(const brew_kv_s* kv, int layer) {
+    KvView v;
+    v.pages = kv->pool + layer * kv->layer_bytes;
+    v.table = kv->table;
+    v.reserved = kv->reserved;
+    v.max_seqs = kv->c.max_seqs;
+    v.max_pages = kv->max_pages;
+    v.page_shift = kv->page_shift;
+    v.n_heads = kv->c.n_heads;
+    v.n_kv = kv->c.n_kv_heads;
+    v.err = kv->err;
+    return v;
+}
+
+bool kv_head_supported(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 256; }
+
+int kv_append_launch(int hd, const KvAppendParams& p, cudaStream_t s) {
+    switch (hd / 32) {
+        case 1: return append_r<1>(p, s);
+        case 2: return append_r<2>(p, s);
+        case 3: return append_r<3>(p, s);
+        case 4: return append_r<4>(p, s);
+        default: return append_r<8>(p, s);
+    }
+}
+
+}  // namespace brew
+
+using namespace brew;
+
+extern "C" {
+
+int brew_kv_create(const brew_kv_config* cfg, brew_kv* out) {
+    BREW_CHECK(cfg && out, BREW_ERR_INVALID_ARG, "null argument");
+    *out = nullptr;
+    const brew_kv_config& c = *cfg;
+    BREW_CHECK(kv_head_supported(c.head_size), BREW_ERR_UNSUPPORTED, "K/V cache: head size %d (32, 64, 96, 128 or 256)",
+               c.head_size);
+    BREW_CHECK(c.n_layers > 0 && c.n_kv_heads > 0 && c.n_heads > 0 && c.n_heads % c.n_kv_heads == 0,
+               BREW_ERR_INVALID_ARG, "K/V cache: %d layers, %d heads, %d kv heads", c.n_layers, c.n_heads, c.n_kv_heads);
+    BREW_CHECK(c.n_heads <= 1024, BREW_ERR_UNSUPPORTED, "K/V cache: %d heads", c.n_heads);
+    BREW_CHECK(c.max_seqs > 0 && c.max_seqs <= KV_MAX_SEQS, BREW_ERR_INVALID_ARG, "K/V cache: %d sequences (1 .. %d)",
+               c.max_seqs, KV_MAX_SEQS);
+    BREW_CHECK(c.max_tokens > 0 && c.max_tokens <= (1 << 30), BREW_ERR_INVALID_ARG, "K/V cache: %d positions a sequence",
+               c.max_tokens);
+    BREW_CHECK(c.page_tokens == 16 || c.page_tokens == 32 || c.page_tokens == 64 || c.page_tokens == 128,
+               BREW_ERR_INVALID_ARG, "K/V cache: pages of %d positions (16, 32, 64 or 128)", c.page_tokens);
+    const int64_t max_pages = ((int64_t)c.max_tokens + c.page_tokens - 1) / c.page_tokens;
+    const int64_t pages = c.n_pages > 0 ? c.n_pages : max_pages * c.max_seqs;
+    BREW_CHECK(c.n_pages >= 0 && pages <= (1 << 30), BREW_ERR_INVALID_ARG, "K/V cache: %lld pages", (long long)pages);
+    const int64_t page_bytes = (int64_t)c.n_kv_heads * (c.page_tokens / KV_GROUP) * kv_group_bytes(c.head_size / 32);
+    BREW_CHECK(pages <= (int64_t)1 << 40 >> 6 && page_bytes * pages <= ((int64_t)1 << 50) / c.n_layers,
+               BREW_ERR_INVALID_ARG, "K/V cache: %lld pages of %lld bytes in %d layers", (long long)pages,
+               (long long)page_bytes, c.n_layers);
+    DeviceScope ds;
+    if (ds.rc) return ds.rc;
+    brew_kv_s* kv = nullptr;
+    try {
+        kv = new brew_kv_s();
+        kv->c = c;
+        kv->c.n_pages = (int32_t)pages;
+        kv->max_pages = (int)max_pages;
+        while ((1 << kv->page_shift) < c.page_tokens) ++kv->page_shift;
+        kv->layer_bytes = page_bytes * pages;
+        kv->device = ctx().device;
+        kv->seq_pages.resize(c.max_seqs);
+        kv->free_pages.resize((size_t)pages);
+        for (int64_t i = 0; i < pages; ++i) kv->free_pages[i] = (int32_t)(pages - 1 - i);
+    } catch (const std::bad_alloc&) {
+        delete kv;
+        return set_error(BREW_ERR_CUDA, "K/V cache: out of host memory");
+    }
+    const size_t tb = sizeof(int32_t) * (size_t)c.max_seqs * max_pages;
+    cudaError_t e = cudaMalloc(&kv->pool, (size_t)kv->layer_bytes * c.n_layers);
+    if (e == cudaSuccess) e = cudaMalloc(&kv->table, tb);
+    if (e == cudaSuccess) e = cudaMalloc(&kv->reserved, sizeof(int32_t) * (c.max_seqs + 1));
+    if (e == cudaSuccess) {
+        kv->err = reinterpret_cast<unsigned int*>(kv->reserved + c.max_seqs);
+        e = cudaMemset(kv->table, 0, tb);
+    }
+    if (e == cudaSuccess) e = cudaMemset(kv->reserved, 0, sizeof(int32_t) * (c.max_seqs + 1));
+    // positions that are reserved and never appended read as zeros
+    if (e == cudaSuccess) e = cudaMemset(kv->pool, 0, (size_t)kv->layer_bytes * c.n_layers);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(0);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        brew_kv_free(kv);
+        return cuda_error(e, "K/V cache allocation");
+    }
+    *out = kv;
+    return BREW_OK;
+}
+
+int brew_kv_free(brew_kv kv) {
+    if (!kv) return BREW_OK;
+    {
+        DeviceScope ds;
+        cudaDeviceSynchronize();
+        cudaFree(kv->pool);
+        cudaFree(kv->table);
+        cudaFree(kv->reserved);
+    }
+    delete kv;
+    return BREW_OK;
+}
+
+int brew_kv_info(brew_kv kv, int64_t* bytes, int32_t* free_pages) {
+    BREW_CHECK(kv, BREW_ERR_INVALID_ARG, "null K/V cache");
+    std::lock_guard<std::mutex> lk(kv->mu);
+    if (bytes) *bytes = kv->layer_bytes * kv->c.n_layers;
+    if (free_pages) *free_pages = (int32_t)kv->free_pages.size();
+    return BREW_OK;
+}
+
+int brew_kv_reserve(brew_kv kv, int32_t seq, int32_t n_tokens, void* stream) {
+    BREW_CHECK(kv, BREW_ERR_INVALID_ARG, "null K/V cache");
+    BREW_CHECK(seq >= 0 && seq < kv->c.max_seqs, BREW_ERR_INVALID_ARG, "sequence %d of %d", seq, kv->c.max_seqs);
+    BREW_CHECK(n_tokens >= 0, BREW_ERR_INVALID_ARG, "%d positions", n_tokens);
+    BREW_CHECK(n_tokens <= kv->c.max_tokens, BREW_ERR_CONTEXT_FULL, "The session has reached its context limit of %d tokens.",
+               kv->c.max_tokens);
+    DeviceScope ds;
+    if (ds.rc) return ds.rc;
+    std::lock_guard<std::mutex> lk(kv->mu);
+    std::vector<int32_t>& have = kv->seq_pages[seq];
+    const size_t need = ((size_t)n_tokens + kv->c.page_tokens - 1) >> kv->page_shift, first = have.size();
+    if (need <= first) return BREW_OK;
+    BREW_CHECK(need - first <= kv->free_pages.size(), BREW_ERR_CONTEXT_FULL,
+               "K/V cache: %zu pages needed, %zu free", need - first, kv->free_pages.size());
+    try {
+        have.reserve(need);
+    } catch (const std::bad_alloc&) {
+        return set_error(BREW_ERR_CUDA, "K/V cache: out of host memory");
+    }
+    for (size_t i = first; i < need; ++i) {
+        have.push_back(kv->free_pages.back());
+        kv->free_pages.pop_back();
+    }
+    return set_pages(kv, seq, first, need, (int)(need << kv->page_shift), static_cast<cudaStream_t>(stream));
+}
+
+int brew_kv_release(brew_kv kv, int32_t seq, void* stream) {
+    BREW_CHECK(kv, BREW_ERR_INVALID_ARG, "null K/V cache");
+    BREW_CHECK(seq >= 0 && seq < kv->c.max_seqs, BREW_ERR_INVALID_ARG, "sequence %d of %d", seq, kv->c.max_seqs);
+    DeviceScope ds;
+    if (ds.rc) return ds.rc;
+    std::lock_guard<std::mutex> lk(kv->mu);
+    std::vector<int32_t>& have = kv->seq_pages[seq];
+    int rc = set_pages(kv, seq, 0, 0, 0, static_cast<cudaStream_t>(stream));
+    if (rc) return rc;
+    // free_pages was sized for every page: no allocation here
+    for (size_t i = have.size(); i-- > 0;) kv->free_pages.push_back(have[i]);
+    have.clear();
+    return BREW_OK;
+}
+
+int brew_kv_append_dev(brew_kv kv, int32_t layer, float* q_out, const float* q, int64_t ldq, const float* k,
+                       const float* v, int64_t ldkv, const brew_kv_rows* rows, const brew_kv_rope* rope, void* stream) {
+    int rc = check_rows(kv, layer, rows);
+    if (rc) return rc;
+    const brew_kv_config& c = kv->c;
+    if ((rc = check_matrix("k", k, ldkv, (int64_t)c.n_kv_heads * c.head_size)) ||
+        (rc = check_matrix("v", v, ldkv, (int64_t)c.n_kv_heads * c.head_size)))
+        return rc;
+    BREW_CHECK((q != nullptr) == (q_out != nullptr), BREW_ERR_INVALID_ARG, "q and q_out are given together");
+    if (q && ((rc = check_matrix("q", q, ldq, (int64_t)c.n_heads * c.head_size)) ||
+              (rc = check_matrix("q_out", q_out, ldq, (int64_t)c.n_heads * c.head_size))))
+        return rc;
+    KvAppendParams p = {};
+    p.rope = BREW_KV_ROPE_NONE;
+    if (rope) {
+        BREW_CHECK(rope->mode == BREW_KV_ROPE_NONE || rope->mode == BREW_KV_ROPE_HALF ||
+                       rope->mode == BREW_KV_ROPE_INTERLEAVED,
+                   BREW_ERR_INVALID_ARG, "rope mode %d", rope->mode);
+        BREW_CHECK(rope->mode == BREW_KV_ROPE_NONE ||
+                       (rope->base > 0.0 && std::isfinite(rope->base) && std::isfinite(rope->scale)),
+                   BREW_ERR_INVALID_ARG, "rope base %g, scale %g", rope->base, rope->scale);
+        const bool norm = rope->qnorm || rope->knorm;
+        BREW_CHECK(!norm || (rope->eps >= 0.0 && std::isfinite(rope->eps)), BREW_ERR_INVALID_ARG, "norm eps %g", rope->eps);
+        BREW_CHECK(((uintptr_t)rope->qnorm & 3) == 0 && ((uintptr_t)rope->knorm & 3) == 0, BREW_ERR_INVALID_ARG,
+                   "unaligned norm weights");
+        p.rope = rope->mode;
+        p.rope_scale = rope->scale;
+        p.log2_base_hd = p.rope == BREW_KV_ROPE_NONE ? 0.0 : std::log2(rope->base) / c.head_size;
+        p.qnorm = rope->qnorm;
+        p.knorm = rope->knorm;
+        p.eps = rope->eps;
+    }
+    if (rows->n_seqs == 0 || rows->n_rows == 0 || rows->max_rows == 0) return BREW_OK;
+    DeviceScope ds;
+    if (ds.rc) return ds.rc;
+    p.kv = kv_view(kv, layer);
+    p.rows = rows_dev(rows);
+    p.q = q;
+    p.q_out = q_out;
+    p.k = k;
+    p.v = v;
+    p.ldq = ldq;
+    p.ldkv = ldkv;
+    return kv_append_launch(c.head_size, p, static_cast<cudaStream_t>(stream));
+}
+
+int brew_kv_read_dev(brew_kv kv, int32_t layer, float* k_out, float* v_out, int64_t ld, const brew_kv_rows* rows,
+                     void* stream) {
+    int rc = check_rows(kv, layer, rows);
+    if (rc) return rc;
+    const brew_kv_config& c = kv->c;
+    BREW_CHECK(k_out || v_out, BREW_ERR_INVALID_ARG, "k_out and v_out are null");
+    if ((k_out && (rc = check_matrix("k_out", k_out, ld, (int64_t)c.n_kv_heads * c.head_size))) ||
+        (v_out && (rc = check_matrix("v_out", v_out, ld, (int64_t)c.n_kv_heads * c.head_size))))
+        return rc;
+    if (rows->n_seqs == 0 || rows->n_rows == 0 || rows->max_rows == 0) return BREW_OK;
+    DeviceScope ds;
+    if (ds.rc) return ds.rc;
+    const KvView view = kv_view(kv, layer);
+    const KvRowsDev rd = rows_dev(rows);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (c.head_size / 32) {
+        case 1: return read_r<1>(view, rd, k_out, v_out, ld, s);
+        case 2: return read_r<2>(view, rd, k_out, v_out, ld, s);
+        case 3: return read_r<3>(view, rd, k_out, v_out, ld, s);
+        case 4: return read_r<4>(view, rd, k_out, v_out, ld, s);
+        default: return read_r<8>(view, rd, k_out, v_out, ld, s);
+    }
+}
+
+int64_t brew_kv_workspace_bytes(brew_kv kv) { return kv ? kv_attend_workspace(kv->c.head_size) : -1; }
+
+int brew_kv_attend_dev(brew_kv kv, int32_t layer, float* out, int64_t ldo, const float* q, int64_t ldq,
+                       const brew_kv_rows* rows, int32_t window, float scale, void* workspace, void* stream) {
+    int rc = check_rows(kv, layer, rows);
+    if (rc) return rc;
+    const brew_kv_config& c = kv->c;
+    if ((rc = check_matrix("out", out, ldo, (int64_t)c.n_heads * c.head_size)) ||
+        (rc = check_matrix("q", q, ldq, (int64_t)c.n_heads * c.head_size)))
+        return rc;
+    BREW_CHECK(window >= 0, BREW_ERR_INVALID_ARG, "window %d", window);
+    BREW_CHECK(std::isfinite(scale), BREW_ERR_INVALID_ARG, "scale %g", (double)scale);
+    BREW_CHECK(workspace && ((uintptr_t)workspace & 255) == 0, BREW_ERR_INVALID_ARG,
+               "the workspace must be given, on a 256-byte boundary");
+    if (rows->n_seqs == 0 || rows->n_rows == 0 || rows->max_rows == 0) return BREW_OK;
+    DeviceScope ds;
+    if (ds.rc) return ds.rc;
+    KvAttendParams p = {};
+    p.kv = kv_view(kv, layer);
+    p.rows = rows_dev(rows);
+    p.q = q;
+    p.out = out;
+    p.ldq = ldq;
+    p.ldo = ldo;
+    p.window = window;
+    p.scale = scale != 0.0f ? scale : 1.0f / (float)std::sqrt((double)c.head_size);   // AttentionEngine.java:18-19
+    p.workspace = workspace;
+    return kv_attend_launch(c.head_size, p, static_cast<cudaStream_t>(stream));
+}
+
+int brew_kv_check(brew_kv kv) {
+    BREW_CHECK(kv, BREW_ERR_INVALID_ARG, "null K/V cache");
+    DeviceScope ds;
+    if (ds.rc) return ds.rc;
+    BREW_CUDA(cudaDeviceSynchronize());
+    unsigned int v = 0;
+    BREW_CUDA(cudaMemcpy(&v, kv->err, sizeof(v), cudaMemcpyDeviceToHost));
+    if (v == 0) return BREW_OK;
+    BREW_CUDA(cudaMemset(kv->err, 0, sizeof(v)));
+    BREW_CUDA(cudaStreamSynchronize(0));
+    if (v & (BREW_DEVERR_TIMEOUT_FULL | BREW_DEVERR_TIMEOUT_EMPTY))
+        return set_error(BREW_ERR_TIMEOUT, "K/V cache: a bounded device wait timed out (flags 0x%x)", v);
+    return set_error(BREW_ERR_OUT_OF_BOUNDS,
+                     "K/V cache: a sequence, position or row outside the cache or its reserved pages was skipped");
+}
+
+}  // extern "C"

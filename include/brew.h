@@ -392,6 +392,117 @@ BREW_API int brew_model_trace(brew_model m, int64_t* ns, int32_t max_n, int32_t*
  * The context stays usable afterwards. */
 BREW_API int brew_selftest_wait_timeout(int64_t limit_ns, int32_t* waits_ended);
 
+/* ---- paged 4-bit K/V cache ------------------------------------------------
+ * No reference counterpart: its RunState keeps fp32 K and V of seq_len
+ * positions for each sequence (RunStateAllocator.java:48-70).  Here k and v
+ * of a position are stored as blocks of 32 values with GGML's Q4_0 rule (d =
+ * -1/8 of the block's first value of largest magnitude, kept as fp16 and at
+ * most 65504 in size; q = trunc(x / d + 8.5) in 0..15; the value is
+ * (q - 8) * d), 0.5625 bytes a value, in pages of page_tokens positions that
+ * sequences take from a common pool.
+ *
+ * brew_kv_reserve gives sequence `seq` the pages of positions 0 ..
+ * n_tokens - 1 (it only grows; BREW_ERR_CONTEXT_FULL past max_tokens or when
+ * the pool is empty, nothing is changed then), brew_kv_release returns them
+ * all.  Both take effect on the device in `stream` order; a page released on
+ * one stream and taken on another needs an ordering between the two.
+ *
+ * The _dev calls take device pointers and enqueue on `stream` (0 = default)
+ * without synchronising or allocating; they can be captured into a CUDA
+ * graph.  A row whose sequence, positions or row numbers lie outside the
+ * cache, its reserved pages or the buffers is skipped (nothing is read or
+ * written for it) and recorded: brew_kv_check synchronises the device,
+ * returns BREW_ERR_OUT_OF_BOUNDS if that happened since the last check, and
+ * forgets it. */
+typedef struct brew_kv_s* brew_kv;
+typedef struct brew_kv_config {
+    int32_t n_layers;
+    int32_t n_heads;        /* query heads, a multiple of n_kv_heads      */
+    int32_t n_kv_heads;
+    int32_t head_size;      /* 32, 64, 96, 128 or 256                     */
+    int32_t max_seqs;       /* sequences 0 .. max_seqs - 1 (at most 2048) */
+    int32_t max_tokens;     /* positions of a sequence                    */
+    int32_t page_tokens;    /* 16, 32, 64 or 128                          */
+    int32_t n_pages;        /* pages of the pool; 0: enough for every sequence's max_tokens */
+} brew_kv_config;
+BREW_API int brew_kv_create(const brew_kv_config* cfg, brew_kv* out);
+BREW_API int brew_kv_free(brew_kv kv);
+BREW_API int brew_kv_info(brew_kv kv, int64_t* bytes, int32_t* free_pages);
+BREW_API int brew_kv_reserve(brew_kv kv, int32_t seq, int32_t n_tokens, void* stream);
+BREW_API int brew_kv_release(brew_kv kv, int32_t seq, void* stream);
+BREW_API int brew_kv_check(brew_kv kv);
+
+/* The rows (tokens) of a call, device arrays of int32: entry i of n_seqs has
+ * rows row_start[i] .. row_start[i + 1] - 1 of the buffers, which are
+ * consecutive positions pos[i], pos[i] + 1, ... of sequence seq[i].
+ * row_start NULL: one row for each entry (row i).  The buffers have n_rows
+ * rows; no entry has more than max_rows.  Entries without rows are allowed,
+ * and rows that no entry has are left as they are.  n_seqs is at most 2048. */
+typedef struct brew_kv_rows {
+    const int32_t* seq;
+    const int32_t* pos;
+    const int32_t* row_start;   /* [n_seqs + 1] or NULL */
+    int32_t n_seqs;
+    int32_t n_rows;
+    int32_t max_rows;
+} brew_kv_rows;
+
+/* What happens to q and k on their way: the head-wise RMSNorm with weights
+ * qnorm / knorm (device [head_size], NULL: none; Kernels.headWiseRmsNorm)
+ * and the rotation of pairs (i, i + head_size / 2) or (2 i, 2 i + 1) by the
+ * angle pos * scale * base^(-2 i / head_size).  Norm, angles and rotation
+ * are computed in 64 bits and rounded once. */
+#define BREW_KV_ROPE_NONE        0
+#define BREW_KV_ROPE_HALF        1
+#define BREW_KV_ROPE_INTERLEAVED 2
+typedef struct brew_kv_rope {
+    int32_t mode;
+    double  base, scale;
+    const float* qnorm;
+    const float* knorm;
+    double  eps;
+} brew_kv_rope;
+
+/* Appends rows: q [n_rows][ldq] (n_heads heads side by side) is normalised
+ * and rotated into q_out (same stride; q_out may be q; both NULL: k and v
+ * only), k likewise and stored, v stored.  rope NULL: neither norm nor
+ * rotation.  A position may be appended again (it is overwritten); no two
+ * rows of a call may be the same position.  Pointers and strides (in floats)
+ * must keep rows on 16-byte boundaries. */
+BREW_API int brew_kv_append_dev(brew_kv kv, int32_t layer, float* q_out, const float* q, int64_t ldq, const float* k,
+                                const float* v, int64_t ldkv, const brew_kv_rows* rows, const brew_kv_rope* rope,
+                                void* stream);
+/* The values that the rows' stored k and v stand for, fp32 [n_rows][ld]
+ * (either output may be NULL). */
+BREW_API int brew_kv_read_dev(brew_kv kv, int32_t layer, float* k_out, float* v_out, int64_t ld,
+                              const brew_kv_rows* rows, void* stream);
+/* out[row] = softmax(scale * q[row] k^T) v for each head over the positions
+ * <= the row's own, of its sequence (the last `window` of them when window >
+ * 0); scale 0 means 1 / sqrt(head_size).  out may not overlap q.  `workspace`:
+ * brew_kv_workspace_bytes(kv) device bytes on a 256-byte boundary,
+ * zero-filled once before its first use (each call leaves it ready for the
+ * next).  Calls and captured graphs that may run at the same time need a
+ * workspace each. */
+BREW_API int64_t brew_kv_workspace_bytes(brew_kv kv);
+BREW_API int brew_kv_attend_dev(brew_kv kv, int32_t layer, float* out, int64_t ldo, const float* q, int64_t ldq,
+                                const brew_kv_rows* rows, int32_t window, float scale, void* workspace, void* stream);
+
+/* ---- token scoring ---------------------------------------------------------
+ * For each row of logits [rows][ld] (device fp32, `vocab` of each row used):
+ * logprob = log softmax(row)[tokens[row]], entropy = -sum p log p (nats), and
+ * the `top` (at most BREW_MAX_TOP) largest entries with their log
+ * probabilities, largest first and equal ones by index, [rows][top].
+ * tokens / logprob, entropy and top_ids / top_logprobs may each be NULL (top
+ * 0).  A token outside the vocabulary has the log probability NaN.  Logits of
+ * -inf have probability 0; a row of nothing else has log probabilities -inf
+ * and entropy 0.  A NaN or +inf makes its row's results NaN (a NaN ranks as
+ * -inf among the alternatives).  No reference counterpart beside
+ * Kernels.argMax (transformer/math/Kernels.java:150-162). */
+#define BREW_MAX_TOP 32
+BREW_API int brew_logprobs_dev(const float* logits, int64_t ld, int32_t vocab, int32_t rows, const int32_t* tokens,
+                               float* logprob, float* entropy, int32_t top, int32_t* top_ids, float* top_logprobs,
+                               void* stream);
+
 /* Clears the sequence state (ModelSession.reset, ModelRunner.java:115-120). */
 BREW_API int brew_model_reset(brew_model m);
 
