@@ -111,6 +111,7 @@ class Filled:
         scale = scale or 1 / math.sqrt(self.hd)
         outs, tols = [], []
         at = 0
+        self.b = 0.0
         for seq, pos, n in entries:
             k = self.k[seq][:pos + n].repeat_interleave(self.group, 1)
             v = self.v[seq][:pos + n].repeat_interleave(self.group, 1)
@@ -122,6 +123,7 @@ class Filled:
             p = torch.softmax(x.masked_fill(dead, -math.inf), -1)
             outs.append(torch.einsum("hrk,khd->rhd", p, v))
             b = torch.einsum("rhd,khd->hrk", qi.abs(), k.abs()).amax() * scale if n and pos + n else 0.0
+            self.b = max(self.b, float(b))
             ds = b * (2 ** -21 + (self.hd + 8) * 2 ** -24)
             tols.append(torch.full((n, 1, 1), float((2 * ds + 2 ** -20 + (pos + n + 64) * 2 ** -24) * v.abs().max())
                                    if n else 0.0, device=DEV))
@@ -132,8 +134,11 @@ class Filled:
         self.kv.check()
         want, tol = self.expected(q, entries, window, scale)
         assert bool(((got - want).abs() <= tol).all()), ((got - want).abs() / tol).max()
-        if want.numel():   # rounding errors are of either sign: far from adding up
-            assert float((got - want).norm() / want.norm().clamp(min=1e-30)) < 1e-5
+        if want.numel():
+            # Rounding errors are of either sign: far from adding up.  But scores near B are numbers with steps of
+            # B 2^-23 in 32 bits (0.012 at B = 10^5, which q of 10^4 reaches), and half a step moves a weight by
+            # B 2^-24 of itself: that much cannot be asked for.
+            assert float((got - want).norm() / want.norm().clamp(min=1e-30)) < 1e-5 + self.b * 2 ** -24
 
 
 # ---- append and read ----------------------------------------------------------------------------------------------------
