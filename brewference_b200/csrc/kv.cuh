@@ -81,6 +81,7 @@ struct KvAttendParams {
     int window;
     float scale;
     void* workspace;
+    uint32_t code_base;        // set by the launch
 };
 
 int kv_append_launch(int head_size, const KvAppendParams& p, cudaStream_t s);

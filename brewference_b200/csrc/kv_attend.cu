@@ -10,10 +10,10 @@
 // head) pairs fill a tile.
 //   scores   S = sum_b d_K[t][b] (sum_{i in b} q_i (c_ti - 8))
 //   output   O = sum_t (p_t d_V[t][b]) (c_ti - 8)
-// q is scaled by a power of two to below 2^14 and p d_V by one that follows
-// the largest |d_V| seen (p d_V <= 2^15), so that neither part leaves fp16's
-// range nor loses bits to its subnormals.  The softmax is online; its running
-// maximum moves only when exceeded by 2^8, so O is rarely rescaled.
+// q, p and d_V are scaled by powers of two (q below 2^14, p and p d_V to 2^15
+// at most), so that no part leaves fp16's range and little falls among its
+// subnormals (2^-24 beside 2^13).  The softmax is online; its running maximum
+// moves only when exceeded by 2^2, so O is rarely rescaled.
 //
 // Work split.  Units of 128 positions of one (sequence, kv head, 8 pairs),
 // laid end to end over all sequences of the call; every CTA takes an equal
@@ -38,7 +38,7 @@ constexpr int AT_TILE = 32;                       // positions a warp handles at
 constexpr int AT_UNIT = AT_TILE * AT_WARPS;
 constexpr int AT_PAIRS = 8;                       // (row, head) pairs of a tile
 constexpr int AT_MAX_CTAS = 3 * 148;
-constexpr float AT_LAZY = 8.0f;                   // log2 of how far p may exceed 1
+constexpr float AT_LAZY = 2.0f;                   // log2 of how far p may exceed 1
 
 template <int R>
 struct AtShape {
@@ -80,11 +80,19 @@ __device__ __forceinline__ void split_half2(float x0, float x1, uint32_t& hi, ui
 // place up 1024 + 16 c); one exact operation takes the rest off.  (A nibble
 // alone, the subnormal c 2^-24, would save that operation, but mma aligns its
 // products by their exponent fields and loses 7 bits of a subnormal's.)
-__device__ __forceinline__ void unpack(uint32_t (&x)[4], uint32_t w) {
+__device__ __forceinline__ uint32_t code_bits(uint32_t w, uint32_t mask, uint32_t base) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(w), "r"(mask), "r"(base));   // w & mask | base
+    return d;
+}
+// `base`: 0x64006400, a launch parameter so that it stays in a register and
+// each step is one instruction (as a constant it took two: 64 more of 478 per
+// 16 positions, and 6 % of the time).
+__device__ __forceinline__ void unpack(uint32_t (&x)[4], uint32_t w, uint32_t base) {
     const uint32_t y = w >> 8;
-    uint32_t e0 = (w & 0x000F000Fu) | 0x64006400u, e1 = (w & 0x00F000F0u) | 0x64006400u;
-    uint32_t e2 = (y & 0x000F000Fu) | 0x64006400u, e3 = (y & 0x00F000F0u) | 0x64006400u;
-    asm("sub.f16x2 %0, %1, %2;" : "=r"(x[0]) : "r"(e0), "r"(0x64086408u));                       // - 1032
+    const uint32_t e0 = code_bits(w, 0x000F000Fu, base), e1 = code_bits(w, 0x00F000F0u, base);
+    const uint32_t e2 = code_bits(y, 0x000F000Fu, base), e3 = code_bits(y, 0x00F000F0u, base);
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(x[0]) : "r"(e0), "r"(0x64086408u));                            // - 1032
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(x[1]) : "r"(e1), "r"(0x2C002C00u), "r"(0xD480D480u));   // / 16 - 72
     asm("sub.f16x2 %0, %1, %2;" : "=r"(x[2]) : "r"(e2), "r"(0x64086408u));
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(x[3]) : "r"(e3), "r"(0x2C002C00u), "r"(0xD480D480u));
@@ -92,6 +100,44 @@ __device__ __forceinline__ void unpack(uint32_t (&x)[4], uint32_t w) {
 
 __device__ __forceinline__ float2 half2_bits(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// Two fp32 numbers at a time.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\t"
+        "mov.b64 {%0, %1}, x;}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+// fp16 pairs.
+__device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t fma_h2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t neg_h2(uint32_t a) {
+    uint32_t d;
+    asm("neg.f16x2 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+// The larger magnitude, with some sign.
+__device__ __forceinline__ uint32_t maxabs_h2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -137,6 +183,24 @@ __device__ __forceinline__ void load_scales(uint32_t (&w)[R], const uint8_t* s, 
     }
 }
 
+// The power of two that d_V is carried with, from the exponent over every
+// |d_V| so far (|d_V| < 2^(ve - 15)): scales all under 2^-6, and those that
+// reach 1, are brought to about 1, so that p d_V times both factors stays
+// under 2^15 and its small terms off fp16's subnormals.
+constexpr float AT_PSCALE = 8192.0f;   // p's factor: p may be 2^AT_LAZY
+struct AtScale {
+    uint32_t ve;     // 1 .. 32
+    uint32_t dmul;   // factor of d_V, an fp16 pair
+    float total;     // both factors
+    __device__ explicit AtScale(uint32_t e) : ve(e) {
+        const int up = e < 10 || e > 15 ? 15 - (int)e : 0;
+        // 2^-15 and less (d_V at fp16's end) are subnormals
+        const uint32_t h = up > -15 ? (uint32_t)(15 + up) << 10 : 1u << (25 + up - 1);
+        dmul = h | h << 16;
+        total = AT_PSCALE * __uint_as_float((uint32_t)(127 + up) << 23);
+    }
+};
+
 // ---- the units of a call ---------------------------------------------------
 struct AtSpan {
     int base;     // first position, rounded down to a tile
@@ -169,6 +233,7 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<R>::CTAS_PER_SM)
     __shared__ int64_t s_warp[AT_WARPS];
     __shared__ int s_last, s_fail;
     const KvView& kv = p.kv;
+    const uint32_t base = p.code_base;
     const int n_kv = kv.n_kv, G = kv.n_heads / n_kv, n_seqs = p.rows.n_seqs;
 
     if (lane == 0) {
@@ -327,9 +392,9 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<R>::CTAS_PER_SM)
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[b][j][c] = 0.0f;
-        float m = -INFINITY, l = 0.0f;
-        int ve = 103;   // float exponent of the largest |d_V|: p d_V is scaled by 2^(133 - ve); fp16's least: 103
-        float vs = __uint_as_float((uint32_t)(260 - 103) << 23);
+        float m = -INFINITY;
+        float2 l2 = make_float2(0.0f, 0.0f);
+        AtScale sv(1);
 
         for (int k = 0; k < nt; ++k) {
             const uint32_t n = it + k, slot = n % S::STAGES;
@@ -342,9 +407,9 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<R>::CTAS_PER_SM)
             const bool full = tpos >= kall_lo && tpos + AT_TILE - 1 <= kall_hi;   // no position is masked
 
             // ---- scores of positions 8 u + 2 i + e (u = 0 .. 3), log2 units
-            float s[4][2];
+            float2 s[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) s[u][0] = s[u][1] = 0.0f;
+            for (int u = 0; u < 4; ++u) s[u] = make_float2(0.0f, 0.0f);
             if constexpr (R == 8) {
                 uint32_t kw[4][8];
                 uint32_t sc[4][8];
@@ -364,13 +429,11 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<R>::CTAS_PER_SM)
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
                         uint32_t x[4];
-                        unpack(x, kw[u][b]);
+                        unpack(x, kw[u][b], base);
                         float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                         mma_f16(c, a[0], x[0], x[1], c);
                         mma_f16(c, a[1], x[2], x[3], c);
-                        const float2 d = half2_bits(sc[u][b]);
-                        s[u][0] = fmaf(d.x, c[0] + c[2], s[u][0]);
-                        s[u][1] = fmaf(d.y, c[1] + c[3], s[u][1]);
+                        s[u] = fma2(half2_bits(sc[u][b]), add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), s[u]);
                     }
                 }
             } else {
@@ -382,41 +445,41 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<R>::CTAS_PER_SM)
 #pragma unroll
                     for (int b = 0; b < R; ++b) {
                         uint32_t x[4];
-                        unpack(x, kw[b]);
+                        unpack(x, kw[b], base);
                         float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                         mma_f16(c, qf[b][0], x[0], x[1], c);
                         mma_f16(c, qf[b][1], x[2], x[3], c);
-                        const float2 d = half2_bits(sc[b]);
-                        s[u][0] = fmaf(d.x, c[0] + c[2], s[u][0]);
-                        s[u][1] = fmaf(d.y, c[1] + c[3], s[u][1]);
+                        s[u] = fma2(half2_bits(sc[b]), add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), s[u]);
                     }
                 }
             }
-            uint32_t dead = 0;   // bit 2 u + e: masked for this lane's pair
             float mx = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s[u] = make_float2(s[u].x * sfac, s[u].y * sfac);
+            uint32_t dead = 0;   // bit 2 u + e: masked for this lane's pair
             if (!full) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int pos = tpos + 8 * u + 2 * i + c;
-                        if (pos > qpos || pos < qlo) dead |= 1u << (2 * u + c);
+                for (int u = 0; u < 4; ++u) {
+                    const int pos = tpos + 8 * u + 2 * i;
+                    if (pos > qpos || pos < qlo) {
+                        dead |= 1u << (2 * u);
+                        s[u].x = -INFINITY;
                     }
+                    if (pos + 1 > qpos || pos + 1 < qlo) {
+                        dead |= 2u << (2 * u);
+                        s[u].y = -INFINITY;
+                    }
+                }
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    s[u][c] = !full && (dead >> (2 * u + c) & 1) ? -INFINITY : s[u][c] * sfac;
-                    mx = fmaxf(mx, s[u][c]);
-                }
+            for (int u = 0; u < 4; ++u) mx = fmaxf(mx, fmaxf(s[u].x, s[u].y));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             if (__any_sync(0xffffffffu, mx > m + AT_LAZY)) {
                 const float mn = mx > m + AT_LAZY ? mx : m;
                 const float corr = mn == m ? 1.0f : ex2(m - mn);   // m = -inf: 0
                 m = mn;
-                l *= corr;
+                l2 = make_float2(l2.x * corr, l2.y * corr);
 #pragma unroll
                 for (int b = 0; b < R; ++b)
 #pragma unroll
@@ -426,40 +489,33 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<R>::CTAS_PER_SM)
             }
             const float mref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    s[u][c] = ex2(s[u][c] - mref);
-                    l += s[u][c];
-                }
+            for (int u = 0; u < 4; ++u) {
+                s[u].x = ex2(s[u].x - mref);
+                s[u].y = ex2(s[u].y - mref);
+                l2 = add2(l2, s[u]);
+            }
 
             // ---- O += (p d_V) (c - 8), a group of 16 positions at a time
+            uint32_t vsc[4][R];
+            uint32_t dm = 0;
 #pragma unroll
-            for (int gr = 0; gr < 2; ++gr) {
-                const uint8_t* grp = tile + gr * kv_group_bytes(R);
-                uint32_t vw[2][R], sc[2][R];
+            for (int u = 0; u < 4; ++u) {
+                load_scales<R>(vsc[u], tile + (u >> 1) * kv_group_bytes(R) + 544 * R, u & 1, i);
+                if (!full) {   // what lies behind a mask may be anything: no NaN of it gets into a product
+                    const uint32_t d2 = dead >> (2 * u);
+                    const uint32_t keep = (d2 & 1 ? 0u : 0xFFFFu) | (d2 & 2 ? 0u : 0xFFFF0000u);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    load_scales<R>(sc[c], grp + 544 * R, c, i);
-                    if (!full) {
-                        const uint32_t d2 = dead >> (4 * gr + 2 * c);
-                        const uint32_t keep = (d2 & 1 ? 0u : 0xFFFFu) | (d2 & 2 ? 0u : 0xFFFF0000u);
-#pragma unroll
-                        for (int b = 0; b < R; ++b) sc[c][b] &= keep;
-                    }
-                    load_words<R>(vw[c], grp + 256 * R, c, lane);
+                    for (int b = 0; b < R; ++b) vsc[u][b] &= keep;
                 }
-                __half2 dm = __float2half2_rn(0.0f);
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int b = 0; b < R; ++b) dm = __hmax2(dm, __habs2(*reinterpret_cast<__half2*>(&sc[c][b])));
-                const float dmax = fmaxf(__low2float(dm), __high2float(dm));
-                if (__any_sync(0xffffffffu, (int)(__float_as_uint(dmax) >> 23) > ve)) {
-                    const int vn = max(ve, (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(dmax)) >> 23));
-                    const float corr = __uint_as_float((uint32_t)max(0, 127 - (vn - ve)) << 23);
-                    ve = vn;
-                    vs = __uint_as_float((uint32_t)(260 - ve) << 23);
+                for (int b = 0; b < R; ++b) dm = maxabs_h2(dm, vsc[u][b]);
+            }
+            {
+                const uint32_t top = max(dm & 0x7FFFu, dm >> 16 & 0x7FFFu) >> 10;   // fp16's exponent field
+                if (__any_sync(0xffffffffu, top >= sv.ve)) {
+                    const AtScale next(__reduce_max_sync(0xffffffffu, top) + 1);
+                    const float corr = next.total * (1.0f / sv.total);
+                    sv = next;
 #pragma unroll
                     for (int b = 0; b < R; ++b)
 #pragma unroll
@@ -467,17 +523,33 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<R>::CTAS_PER_SM)
 #pragma unroll
                             for (int c = 0; c < 4; ++c) o[b][j][c] *= corr;
                 }
-                const float p00 = s[2 * gr][0] * vs, p01 = s[2 * gr][1] * vs;
-                const float p10 = s[2 * gr + 1][0] * vs, p11 = s[2 * gr + 1][1] * vs;
+                if (sv.dmul != 0x3C003C00u) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+#pragma unroll
+                        for (int b = 0; b < R; ++b) vsc[u][b] = mul_h2(vsc[u][b], sv.dmul);
+                }
+            }
+#pragma unroll
+            for (int gr = 0; gr < 2; ++gr) {
+                const uint8_t* grp = tile + gr * kv_group_bytes(R);
+                uint32_t vw[2][R], ph[2], pl[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    load_words<R>(vw[c], grp + 256 * R, c, lane);
+                    split_half2(s[2 * gr + c].x * AT_PSCALE, s[2 * gr + c].y * AT_PSCALE, ph[c], pl[c]);
+                }
 #pragma unroll
                 for (int b = 0; b < R; ++b) {
-                    const float2 d0 = half2_bits(sc[0][b]), d1 = half2_bits(sc[1][b]);
+                    // p d as two fp16 numbers: the rounded ph d, and its exact rest plus pl d
                     uint32_t a[4];
-                    split_half2(p00 * d0.x, p01 * d0.y, a[0], a[1]);
-                    split_half2(p10 * d1.x, p11 * d1.y, a[2], a[3]);
+                    a[0] = mul_h2(ph[0], vsc[2 * gr][b]);
+                    a[1] = fma_h2(pl[0], vsc[2 * gr][b], fma_h2(ph[0], vsc[2 * gr][b], neg_h2(a[0])));
+                    a[2] = mul_h2(ph[1], vsc[2 * gr + 1][b]);
+                    a[3] = fma_h2(pl[1], vsc[2 * gr + 1][b], fma_h2(ph[1], vsc[2 * gr + 1][b], neg_h2(a[2])));
                     uint32_t x0[4], x1[4];
-                    unpack(x0, vw[0][b]);
-                    unpack(x1, vw[1][b]);
+                    unpack(x0, vw[0][b], base);
+                    unpack(x1, vw[1][b], base);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) mma_f16(o[b][j], a, x0[j], x1[j], o[b][j]);
                 }
@@ -489,11 +561,12 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<R>::CTAS_PER_SM)
         it += nt;
 
         // ---- the warps' results meet in shared memory (each in its own ring)
+        float l = l2.x + l2.y;
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         float* mine = reinterpret_cast<float*>(ring);   // [pairs][HD], then [pairs][2]
         {
-            const float un = 1.0f / vs;
+            const float un = 1.0f / sv.total;
 #pragma unroll
             for (int b = 0; b < R; ++b)
 #pragma unroll
@@ -604,7 +677,9 @@ int attend_r(const KvAttendParams& p, cudaStream_t s) {
         BREW_CUDA(smem_attr_per_device((const void*)kv_attend_kernel<R>, S::PREFIX + 8 * (KV_MAX_SEQS + 1), &done));
     }
     const int ctas = std::min(AT_MAX_CTAS, S::CTAS_PER_SM * num_sms());
-    kv_attend_kernel<R><<<ctas, AT_THREADS, smem, s>>>(p);
+    KvAttendParams q = p;
+    q.code_base = 0x64006400u;
+    kv_attend_kernel<R><<<ctas, AT_THREADS, smem, s>>>(q);
     BREW_CUDA(cudaGetLastError());
     count_launch();
     return BREW_OK;
