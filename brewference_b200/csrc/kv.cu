@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(const __grid_cons
             }
             if ((l & 7) == 0) {
                 uint16_t* sc = reinterpret_cast<uint16_t*>(grp + 512 * R + (isk ? 0 : 32 * R));
-                sc[kv_scale(R, pg, b)] = __half_as_ushort(__float2half_rn(d));
+                sc[isk ? kv_kscale(R, pg, b) : kv_vscale(R, pg, b)] = __half_as_ushort(__float2half_rn(d));
             }
         }
     }
@@ -223,10 +223,10 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
         const int64_t o = (e.row0 + j) * ld + (int64_t)hk * 32 * R + 4 * d4;
         const uint16_t* kq = reinterpret_cast<const uint16_t*>(grp);
         const uint16_t* sc = reinterpret_cast<const uint16_t*>(grp + 512 * R);
-        const int si = kv_scale(R, pg, b);
         const uint32_t qk = kq[2 * kv_word(R, u, b, (pg & 7) * 4 + l / 2) + (l & 1)];
         const uint32_t qv = kq[128 * R + 2 * kv_word(R, u, b, l * 4 + ((pg & 7) >> 1)) + (pg & 1)];
-        const float dk = half_bits_to_float(sc[si]), dv = half_bits_to_float(sc[16 * R + si]);
+        const float dk = half_bits_to_float(sc[kv_kscale(R, pg, b)]);
+        const float dv = half_bits_to_float(sc[16 * R + kv_vscale(R, pg, b)]);
         auto val = [](uint32_t q, int c, float d) { return (float)((int)(q >> 4 * c & 15) - 8) * d; };
         if (k_out)
             *reinterpret_cast<float4*>(k_out + o) = make_float4(val(qk, 0, dk), val(qk, 1, dk), val(qk, 2, dk), val(qk, 3, dk));

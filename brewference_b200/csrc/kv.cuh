@@ -15,7 +15,8 @@
 //   K word (u, b, lane)   position 8 u + g, dims 32 b + 8 i + n in nibble n
 //   V word (u, b, lane)   positions 8 u + 2 i + e in 16-bit half e, dims
 //                         32 b + 4 g + j in the half's nibble j
-//   scales                fp16, ((p / 2) R + b) 2 + p % 2: a position pair's
+//   K scales              fp16, p R + b: a position's side by side
+//   V scales              fp16, ((p / 2) R + b) 2 + p % 2: a position pair's
 //                         scales of one block side by side
 //
 // A nibble q stands for (q - 8) * scale: the values of GGML's Q4_0 blocks.
@@ -37,7 +38,8 @@ __host__ __device__ constexpr int kv_word(int R, int u, int b, int lane) {
     return ((m / W) * 32 + lane) * W + m % W;
 }
 
-__host__ __device__ constexpr int kv_scale(int R, int p, int b) { return ((p >> 1) * R + b) * 2 + (p & 1); }
+__host__ __device__ constexpr int kv_kscale(int R, int p, int b) { return p * R + b; }
+__host__ __device__ constexpr int kv_vscale(int R, int p, int b) { return ((p >> 1) * R + b) * 2 + (p & 1); }
 
 // The cache as the kernels see it, one layer.
 struct KvView {

@@ -4,10 +4,10 @@
 //
 // Arithmetic.  A cached value is (c - 8) d with a 4-bit code c and an fp16
 // scale d of its block of 32.  Both products run on mma.m16n8k16 with the
-// codes' exact c - 8 as one operand.  fp32 accuracy comes from the other
-// operand, carried as two fp16 numbers (hi = fp16(x), lo = fp16(x - hi), 22
-// bits together) in rows g and g + 8 of the tile, summed in fp32; 8 (row,
-// head) pairs fill a tile.
+// codes' exact c - 8 as the 16-row operand (16 positions, or 16 dims) and 8
+// (row, head) pairs as the 8 columns.  fp32 accuracy comes from carrying the
+// other operand as two fp16 numbers (hi = fp16(x), lo = fp16(x - hi), 22 bits
+// together), one product each.
 //   scores   S = sum_b d_K[t][b] (sum_{i in b} q_i (c_ti - 8))
 //   output   O = sum_t (p_t d_V[t][b]) (c_ti - 8)
 // q, p and d_V are scaled by powers of two (q below 2^14, p and p d_V to 2^15
@@ -15,14 +15,15 @@
 // subnormals (2^-24 beside 2^13).  The softmax is online; its running maximum
 // moves only when exceeded by 2^2, so O is rarely rescaled.
 //
-// Work split.  Units of 128 positions of one (sequence, kv head, 8 pairs),
+// Work split.  Units of a tile for each warp of one (sequence, kv head, 8 pairs),
 // laid end to end over all sequences of the call; every CTA takes an equal
 // run of units, whatever the lengths (read on the device: a captured graph
 // follows them).  A run's first and last item may be shared with other CTAs:
 // their partial results (max, sum, O) go to the workspace and the last CTA to
-// arrive joins them in order.  Within a unit each warp streams its own
+// arrive joins them in order.  Within an item each warp streams its own
 // 32-position tiles through a ring of shared-memory stages (bulk copies: the
-// tile's K, V and scales are one run per page).
+// tile's K, V and scales are one run per page); the next item's first tiles
+// are under way while an item's warps meet.
 #include <algorithm>
 
 #include "brew_internal.cuh"
@@ -32,34 +33,50 @@
 namespace brew {
 namespace {
 
-constexpr int AT_WARPS = 4;
-constexpr int AT_THREADS = 32 * AT_WARPS;
 constexpr int AT_TILE = 32;                       // positions a warp handles at once
-constexpr int AT_UNIT = AT_TILE * AT_WARPS;
 constexpr int AT_PAIRS = 8;                       // (row, head) pairs of a tile
-constexpr int AT_MAX_CTAS = 3 * 148;
+constexpr int AT_MAX_CTAS = 4 * 148;
+// mma truncates as it accumulates: after this many tiles its sums are added,
+// rounded, to others (128 x 8192 positions: error 3.0e-6 without).
+constexpr int AT_FLUSH = 8;
 constexpr float AT_LAZY = 2.0f;                   // log2 of how far p may exceed 1
 
 template <int R>
 struct AtShape {
     static constexpr int HD = 32 * R;
+    // 16 warps an SM (8 with heads of 256)
+    static constexpr int WARPS = R == 8 || R == 4 ? 8 : 4;
+    static constexpr int CTAS_PER_SM = R == 8 ? 1 : R == 4 ? 2 : 4;
+    static constexpr int THREADS = 32 * WARPS;
+    static constexpr int UNIT = AT_TILE * WARPS;
     static constexpr int TILE_BYTES = 2 * kv_group_bytes(R);
-    static constexpr int STAGES = R <= 2 ? 6 : R == 3 ? 5 : R == 4 ? 4 : 3;
-    static constexpr int RING = STAGES * TILE_BYTES;               // of a warp
-    static constexpr int QFRAG = R == 8 ? R * 2 * 32 * 16 : 0;     // q fragments in shared memory
-    static constexpr int BARS = AT_WARPS * RING + QFRAG;
-    static constexpr int PREFIX = BARS + AT_WARPS * STAGES * 8;
-    static constexpr int CTAS_PER_SM = R == 8 ? 2 : 3;
-    static_assert(AT_PAIRS * (HD + 2) * 4 <= RING, "a warp's result fits its ring");
+    static constexpr int STAGES = R <= 2 ? 4 : 2;
+    static constexpr int RING = STAGES * TILE_BYTES;   // of a warp
+    static constexpr int PITCH = HD + 4;               // floats of a pair's result (conflict-free stores)
+    static constexpr int SUMS = (AT_PAIRS * PITCH + 2 * AT_PAIRS) * 4;   // of a warp: its sums, later its result
+    static constexpr int Q = WARPS * (RING + SUMS);
+    static constexpr int QBYTES = R * 2 * 32 * 16 + AT_PAIRS * 4;        // q's fragments, the pairs' factors
+    static constexpr int BARS = Q + QBYTES;
+    static constexpr int PREFIX = BARS + WARPS * STAGES * 8;
+    static_assert(SUMS % 16 == 0 && RING % 128 == 0, "alignment");
+    static_assert(AT_MAX_CTAS * 4 <= RING, "a join's weights fit a warp's ring");
 };
 
 // ---- mma.m16n8k16 --------------------------------------------------------
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
                                         const float (&c)[4]) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
+// The first product of a sum.
+__device__ __forceinline__ void mma_f16_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{0f00000000,0f00000000,0f00000000,0f00000000};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
@@ -98,10 +115,6 @@ __device__ __forceinline__ void unpack(uint32_t (&x)[4], uint32_t w, uint32_t ba
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(x[3]) : "r"(e3), "r"(0x2C002C00u), "r"(0xD480D480u));
 }
 
-__device__ __forceinline__ float2 half2_bits(uint32_t w) {
-    return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-
 // Two fp32 numbers at a time.
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 d;
@@ -109,14 +122,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         "mov.b64 {%0, %1}, x;}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
-        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-
 // fp16 pairs.
 __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
     uint32_t d;
@@ -187,51 +192,99 @@ __device__ __forceinline__ void load_scales(uint32_t (&w)[R], const uint8_t* s, 
 // |d_V| so far (|d_V| < 2^(ve - 15)): scales all under 2^-6, and those that
 // reach 1, are brought to about 1, so that p d_V times both factors stays
 // under 2^15 and its small terms off fp16's subnormals.
-constexpr float AT_PSCALE = 8192.0f;   // p's factor: p may be 2^AT_LAZY
+constexpr float AT_PLOG2 = 13.0f;   // p is carried times 2^13, sums and all: p may be 2^AT_LAZY
 struct AtScale {
     uint32_t ve;     // 1 .. 32
     uint32_t dmul;   // factor of d_V, an fp16 pair
-    float total;     // both factors
+    float total;     // the same, fp32
     __device__ explicit AtScale(uint32_t e) : ve(e) {
         const int up = e < 10 || e > 15 ? 15 - (int)e : 0;
         // 2^-15 and less (d_V at fp16's end) are subnormals
         const uint32_t h = up > -15 ? (uint32_t)(15 + up) << 10 : 1u << (25 + up - 1);
         dmul = h | h << 16;
-        total = AT_PSCALE * __uint_as_float((uint32_t)(127 + up) << 23);
+        total = __uint_as_float((uint32_t)(127 + up) << 23);
     }
 };
+
+// An 8 x 8 matrix of fp16, row g in lanes 4 g .. 4 g + 3, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// K scales of position p of a group, blocks 0 .. R - 1.
+template <int R>
+__device__ __forceinline__ void load_kscales(__half (&d)[R], const uint8_t* s, int p) {
+    const uint8_t* q = s + 2 * R * p;
+    if constexpr (R % 4 == 0) {
+#pragma unroll
+        for (int c = 0; c < R / 4; ++c) {
+            const uint2 v = *reinterpret_cast<const uint2*>(q + 8 * c);
+            const __half2 a = *reinterpret_cast<const __half2*>(&v.x), b = *reinterpret_cast<const __half2*>(&v.y);
+            d[4 * c] = __low2half(a); d[4 * c + 1] = __high2half(a);
+            d[4 * c + 2] = __low2half(b); d[4 * c + 3] = __high2half(b);
+        }
+    } else if constexpr (R == 2) {
+        const __half2 a = *reinterpret_cast<const __half2*>(q);
+        d[0] = __low2half(a); d[1] = __high2half(a);
+    } else {
+#pragma unroll
+        for (int b = 0; b < R; ++b) d[b] = *reinterpret_cast<const __half*>(q + 2 * b);
+    }
+}
 
 // ---- the units of a call ---------------------------------------------------
 struct AtSpan {
     int base;     // first position, rounded down to a tile
-    int units;    // of AT_UNIT positions
+    int units;    // of AtShape::UNIT positions
     int groups;   // of AT_PAIRS (row, head) pairs
 };
 
+template <int R>
 __device__ __forceinline__ AtSpan at_span(const KvEntry& e, int window, int G) {
     const int first = window > 0 ? max(0, e.pos0 - window + 1) : 0;
     AtSpan s;
     s.base = first & ~(AT_TILE - 1);
-    s.units = (e.pos0 + e.rows - 1 - s.base) / AT_UNIT + 1;
+    s.units = (e.pos0 + e.rows - 1 - s.base) / AtShape<R>::UNIT + 1;
     s.groups = (int)(((int64_t)e.rows * G + AT_PAIRS - 1) / AT_PAIRS);
     return s;
 }
 
-// First CTA whose run reaches past unit u: CTA c has units floor(U c / C) ..
+// The CTA of unit u: CTA c has units U c / C up to U (c + 1) / C
 __device__ __forceinline__ int cta_of(int64_t u, int64_t U, int C) { return (int)(((u + 1) * C + U - 1) / U) - 1; }
 
+__host__ __device__ constexpr int at_part_floats(int HD) { return AT_PAIRS * (HD + 2); }   // O, then (max, sum)
+constexpr int AT_COUNTER_BYTES = (AT_MAX_CTAS * 4 + 255) / 256 * 256;
+
+// A CTA's run through one item.
+struct AtSeg {
+    int seq, pos0, row0;
+    int hk, pr0, npairs;
+    int ua, ub, units;        // units [ua, ub) of the item's
+    int64_t item0;            // the item's first unit
+    int t0, nt;               // first tile of this warp (tiles of a unit are dealt to the warps), and how many
+    int kmax;                 // last position that a pair sees
+    int all_lo, all_hi;       // positions that all pairs see
+};
+
 template <int R>
-__global__ void __launch_bounds__(AT_THREADS, AtShape<R>::CTAS_PER_SM)
+__global__ void __launch_bounds__(AtShape<R>::THREADS, AtShape<R>::CTAS_PER_SM)
     kv_attend_kernel(const __grid_constant__ KvAttendParams p) {
     using S = AtShape<R>;
     constexpr int HD = S::HD;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, i = lane & 3;
     uint8_t* ring = smem + warp * S::RING;
+    float* mine = reinterpret_cast<float*>(smem + S::WARPS * S::RING + warp * S::SUMS);
+    uint4* qs = reinterpret_cast<uint4*>(smem + S::Q);                 // [block][hi, lo][lane]
+    float* qfac = reinterpret_cast<float*>(smem + S::Q + R * 2 * 32 * 16);   // [pair]
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BARS) + warp * S::STAGES;
-    int64_t* prefix = reinterpret_cast<int64_t*>(smem + S::PREFIX);   // [n_seqs + 1]
-    __shared__ int64_t s_warp[AT_WARPS];
-    __shared__ int s_last, s_fail;
+    int64_t* prefix = reinterpret_cast<int64_t*>(smem + S::PREFIX);   // [a thread's entries]
+    __shared__ int64_t s_warp[S::WARPS];
+    __shared__ AtSeg s_seg[S::WARPS], s_done;   // the warps' present item, and the one whose result is made
+    __shared__ AtSeg s_ends[2];            // the run's first and last item, where shared with other CTAs
+    __shared__ int s_fail, s_join[2];
     const KvView& kv = p.kv;
     const uint32_t base = p.code_base;
     const int n_kv = kv.n_kv, G = kv.n_heads / n_kv, n_seqs = p.rows.n_seqs;
@@ -240,18 +293,19 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<R>::CTAS_PER_SM)
         for (int k = 0; k < S::STAGES; ++k) mbar_init(&bars[k], 1);
         fence_mbar_init();
     }
-    // units before each entry
-    int64_t carry = 0;
-    for (int b0 = 0; b0 < n_seqs; b0 += AT_THREADS) {
-        const int k = b0 + tid;
+    if (tid == 0) s_fail = 0;
+    // units before each thread's entries (one for up to 256 of them)
+    auto entry_units = [&](const KvEntry& e) -> int64_t {
+        if (e.rows <= 0) return 0;
+        const AtSpan sp = at_span<R>(e, p.window, G);
+        return (int64_t)sp.units * sp.groups * n_kv;
+    };
+    const int step = (n_seqs + S::THREADS - 1) / S::THREADS, nsteps = (n_seqs + step - 1) / step;
+    int64_t U = 0;
+    {
         int64_t n = 0;
-        if (k < n_seqs) {
-            const KvEntry e = kv_entry(kv, p.rows, k, blockIdx.x == 0);
-            if (e.rows > 0) {
-                const AtSpan sp = at_span(e, p.window, G);
-                n = (int64_t)sp.units * sp.groups * n_kv;
-            }
-        }
+        for (int k = tid * step; k < min(n_seqs, (tid + 1) * step); ++k)
+            n += entry_units(kv_entry(kv, p.rows, k, blockIdx.x == 0));
         int64_t inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -260,351 +314,407 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<R>::CTAS_PER_SM)
         }
         if (lane == 31) s_warp[warp] = inc;
         __syncthreads();
-        int64_t before = carry;
-        for (int w = 0; w < warp; ++w) before += s_warp[w];
-        if (k < n_seqs) prefix[k] = before + inc - n;
-        for (int w = 0; w < AT_WARPS; ++w) carry += s_warp[w];
+        int64_t before = 0;
+#pragma unroll
+        for (int w = 0; w < S::WARPS; ++w) {
+            if (w < warp) before += s_warp[w];
+            U += s_warp[w];
+        }
+        if (tid < nsteps) prefix[tid] = before + inc - n;
         __syncthreads();
     }
-    const int64_t U = carry;
-    if (tid == 0) {
-        prefix[n_seqs] = U;
-        s_fail = 0;
-    }
-    __syncthreads();
-    if (U == 0) return;
     const int C = (int)min((int64_t)gridDim.x, U), cta = blockIdx.x;
     if (cta >= C) return;
     const int64_t u_begin = U * cta / C, u_end = U * (cta + 1) / C;
 
-    int* counters = reinterpret_cast<int*>(p.workspace);
-    float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + 4096);   // [CTA][2][pairs][HD + 2]
-    constexpr int PART = AT_PAIRS * (HD + 2);
-    uint32_t it = 0;   // tiles this warp has taken from its ring
-
-    for (int64_t u = u_begin; u < u_end;) {
-        int lo = 0, hi = n_seqs;   // the entry of unit u: prefix[lo] <= u < prefix[hi]
+    auto locate = [&](int64_t u, AtSeg& to) {
+        int lo = 0, hi = nsteps;   // the entries of unit u: prefix[lo] <= u, the next one's is more
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (prefix[mid] <= u) lo = mid;
             else hi = mid;
         }
-        const KvEntry e = kv_check_entry(kv, p.rows, lo);
-        if (e.rows == 0) break;   // its arrays changed under the kernel
-        const AtSpan sp = at_span(e, p.window, G);
-        const int64_t rel = u - prefix[lo];
-        const int item = (int)(rel / sp.units), ua = (int)(rel - (int64_t)item * sp.units);
-        const int ub = (int)min((int64_t)sp.units, ua + (u_end - u));
-        const int hk = item / sp.groups, pr0 = (item - hk * sp.groups) * AT_PAIRS;
-        const int npairs = min(AT_PAIRS, (int)min((int64_t)e.rows * G - pr0, (int64_t)AT_PAIRS));
-        const int jmin = pr0 / G, jmax = (pr0 + npairs - 1) / G;
-        // positions that some pair sees, and those that all pairs see
-        const int kmax = e.pos0 + jmax, kall_hi = e.pos0 + jmin;
-        const int kmin = p.window > 0 ? max(0, kall_hi - p.window + 1) : 0;
-        const int kall_lo = p.window > 0 ? max(0, kmax - p.window + 1) : 0;
-        const int t0 = max(sp.base / AT_TILE + ua * AT_WARPS, kmin / AT_TILE);
-        const int t1 = min(sp.base / AT_TILE + ub * AT_WARPS, kmax / AT_TILE + 1);
-        const int nt = t0 + warp < t1 ? (t1 - t0 - warp + AT_WARPS - 1) / AT_WARPS : 0;
-        // this lane's pair (a missing one computes the last one's again)
-        const int pi = pr0 + min(g, npairs - 1), jr = pi / G;
-        const int qpos = e.pos0 + jr, qlo = p.window > 0 ? qpos - p.window + 1 : 0;
+        AtSeg s;
+        int64_t rel = u - prefix[lo];
+        int k = lo * step;
+        KvEntry e = kv_check_entry(kv, p.rows, k);
+        for (int64_t n; k + 1 < n_seqs && rel >= (n = entry_units(e)); rel -= n) e = kv_check_entry(kv, p.rows, ++k);
+        AtSpan sp = {0, 1, 1};
+        if (e.rows > 0) sp = at_span<R>(e, p.window, G);
+        const int item = rel < (1ll << 31) ? (int)rel / sp.units : (int)(rel / sp.units);
+        s.seq = e.seq;
+        s.pos0 = e.pos0;
+        s.row0 = e.row0;
+        s.units = sp.units;
+        s.ua = (int)(rel - (int64_t)item * sp.units);
+        s.ub = (int)min((int64_t)sp.units, s.ua + (u_end - u));
+        s.item0 = u - s.ua;
+        s.hk = item / sp.groups;
+        s.pr0 = (item - s.hk * sp.groups) * AT_PAIRS;
+        s.npairs = (int)min((int64_t)e.rows * G - s.pr0, (int64_t)AT_PAIRS);
+        s.all_hi = e.pos0 + s.pr0 / G;                       // the first pair's position
+        s.kmax = e.pos0 + (s.pr0 + s.npairs - 1) / G;        // the last one's
+        s.all_lo = p.window > 0 ? max(0, s.kmax - p.window + 1) : 0;
+        const int kmin = p.window > 0 ? max(0, s.all_hi - p.window + 1) : 0;
+        const int a = max(sp.base / AT_TILE + s.ua * S::WARPS, kmin / AT_TILE) + warp;
+        const int b = min(sp.base / AT_TILE + s.ub * S::WARPS, s.kmax / AT_TILE + 1);
+        s.t0 = a;
+        s.nt = e.rows > 0 && a < b ? (b - a + S::WARPS - 1) / S::WARPS : 0;
+        if (lane == 0) to = s;
+    };
 
-        // ---- copies: page ids of 32 of this warp's tiles at a time, one a lane
-        const int32_t* pages = kv.table + (int64_t)e.seq * kv.max_pages;
-        const int per = 1 << (kv.page_shift - 4);
-        int id0 = 0, id1 = 0;
-        auto lookup = [&](int k0) {
-            const int pos = (t0 + warp + (k0 + lane) * AT_WARPS) * AT_TILE;
-            if (k0 + lane < nt) {
-                id0 = pages[pos >> kv.page_shift];
-                if (kv.page_shift == 4 && pos + 16 <= kmax) id1 = pages[(pos >> 4) + 1];
-            }
-        };
-        auto issue = [&](int k) {   // the warp's tile k into its next stage
-            const int pos = (t0 + warp + k * AT_WARPS) * AT_TILE;
-            const int p0 = __shfl_sync(0xffffffffu, id0, k & 31), p1 = __shfl_sync(0xffffffffu, id1, k & 31);
-            if (lane == 0) {
-                const uint32_t slot = (it + k) % S::STAGES;   // `it` is the segment's first
-                uint8_t* dst = ring + slot * S::TILE_BYTES;
-                const bool two = pos + 16 <= kmax;   // the second group holds a position that is seen
-                const uint32_t bytes = kv_group_bytes(R) * (two ? 2 : 1);
-                mbar_arrive_expect_tx(&bars[slot], bytes);
-                const int64_t g0 = ((int64_t)p0 * n_kv + hk) * per + ((pos >> 4) & (per - 1));
-                if (kv.page_shift > 4) {
-                    bulk_g2s(dst, kv.pages + g0 * kv_group_bytes(R), bytes, &bars[slot]);
-                } else {
-                    bulk_g2s(dst, kv.pages + g0 * kv_group_bytes(R), kv_group_bytes(R), &bars[slot]);
-                    if (two)
-                        bulk_g2s(dst + kv_group_bytes(R), kv.pages + ((int64_t)p1 * n_kv + hk) * kv_group_bytes(R),
-                                 kv_group_bytes(R), &bars[slot]);
-                }
-            }
-        };
-        lookup(0);
-        for (int k = 0; k < min(nt, S::STAGES); ++k) issue(k);
+    // ---- copies: the sources of 32 of this warp's tiles at a time, one a
+    // lane, which issues them itself when their turn comes
+    const int per = 1 << (kv.page_shift - 4);   // groups of a page and head
+    const uint8_t *src0 = nullptr, *src1 = nullptr;
+    uint32_t nbytes = 0;
+    auto lookup = [&](const AtSeg& s, int k0) {
+        const int pos = (s.t0 + (k0 + lane) * S::WARPS) * AT_TILE;
+        if (k0 + lane < s.nt) {
+            const int32_t* pages = kv.table + (int64_t)s.seq * kv.max_pages;
+            const int id = pages[pos >> kv.page_shift];
+            src0 = kv.pages + (((int64_t)id * n_kv + s.hk) * per + ((pos >> 4) & (per - 1))) * kv_group_bytes(R);
+            const bool two = pos + 16 <= s.kmax;   // the second group holds a position that is seen
+            nbytes = kv_group_bytes(R) * (two ? 2 : 1);
+            if (per == 1 && two)
+                src1 = kv.pages + ((int64_t)pages[(pos >> 4) + 1] * n_kv + s.hk) * kv_group_bytes(R);
+        }
+    };
+    auto issue = [&](int k, uint32_t n) {   // tile k, the warp's n-th, into its stage
+        if (lane == (k & 31)) {
+            const uint32_t slot = n % S::STAGES;
+            uint8_t* dst = ring + slot * S::TILE_BYTES;
+            mbar_arrive_expect_tx(&bars[slot], nbytes);
+            bulk_g2s(dst, src0, per > 1 ? nbytes : kv_group_bytes(R), &bars[slot]);
+            if (per == 1 && nbytes > kv_group_bytes(R))
+                bulk_g2s(dst + kv_group_bytes(R), src1, kv_group_bytes(R), &bars[slot]);
+        }
+    };
+    uint32_t nth = 0;   // tiles this warp has taken
+    auto fill = [&](const AtSeg& s) {
+        lookup(s, 0);
+        for (int k = 0; k < min(s.nt, S::STAGES); ++k) issue(k, nth + k);
+    };
 
-        // ---- q: two fp16 parts of the pair's vector times a power of two
-        float sfac;                       // score = sfac * (sum of the products)
-        uint32_t qf[R == 8 ? 1 : R][2][4];
-        uint4* qs = reinterpret_cast<uint4*>(smem + AT_WARPS * S::RING);
-        {
-            const float* qr = p.q + (int64_t)(e.row0 + jr) * p.ldq + (int64_t)(hk * G + pi - jr * G) * HD + 8 * i;
+    int* counters = reinterpret_cast<int*>(p.workspace);                                             // [CTA]
+    float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + AT_COUNTER_BYTES);   // [CTA][2][part]
+    AtSeg& seg = s_seg[warp];
+    const AtSeg& done = s_done;
+    locate(u_begin, seg);
+    __syncwarp();
+    fill(seg);
+    bool split_first = false, split_last = false;   // the run's first and last item is shared
+
+    for (int64_t u = u_begin;;) {
+        // ---- q: a warp makes a pair's two fp16 parts, times a power of two
+        for (int pair = warp; pair < AT_PAIRS; pair += S::WARPS) {
+            const int pi = seg.pr0 + min(pair, seg.npairs - 1), j = pi / G;   // missing pairs repeat the last one
+            const float* qr = p.q + (int64_t)(seg.row0 + j) * p.ldq + (int64_t)(seg.hk * G + pi - j * G) * HD;
+            constexpr int NV = R == 8 ? 2 : 1;
+            float4 x[NV];
             float amax = 0.0f;
 #pragma unroll
-            for (int b = 0; b < R; ++b)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const float4 x = *reinterpret_cast<const float4*>(qr + 32 * b + 4 * c);
-                    amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-                }
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            for (int n = 0; n < NV; ++n) {
+                x[n] = 4 * lane < HD ? *reinterpret_cast<const float4*>(qr + 128 * n + 4 * lane) : make_float4(0, 0, 0, 0);
+                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x[n].x), fabsf(x[n].y)), fmaxf(fabsf(x[n].z), fabsf(x[n].w))));
+            }
+            amax = warp_max(amax);
             // amax * f in [2^13, 2^14)
             const int fe = min(253, max(1, 267 - (int)(__float_as_uint(amax) >> 23)));
-            const float f = __uint_as_float((uint32_t)fe << 23);
-            sfac = p.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(254 - fe) << 23);
+            const float f = copysignf(__uint_as_float((uint32_t)fe << 23), p.scale);   // a negative scale turns q
+            // (never 0: a masked score is -inf times it)
+            if (lane == 0)
+                qfac[pair] = fmaxf(fabsf(p.scale) * 1.44269504088896341f * __uint_as_float((uint32_t)(254 - fe) << 23), 1e-37f);
 #pragma unroll
-            for (int b = 0; b < R; ++b) {
-                const float4 x = *reinterpret_cast<const float4*>(qr + 32 * b);
-                const float4 y = *reinterpret_cast<const float4*>(qr + 32 * b + 4);
-                const float v[8] = {x.x * f, x.y * f, x.z * f, x.w * f, y.x * f, y.y * f, y.z * f, y.w * f};
-                // k order of the two products: nibbles (0, 4 | 1, 5) and (2, 6 | 3, 7)
-                uint32_t a[2][4];
+            for (int n = 0; n < NV; ++n) {
+                // dims 8 i + 0 .. 3 (even lanes) and 8 i + 4 .. 7 (odd) of block b; k order of the products: dims
+                // (0, 4 | 1, 5) and (2, 6 | 3, 7); the even lane stores the high parts, the odd one the low ones
+                const float v[4] = {x[n].x * f, x[n].y * f, x[n].z * f, x[n].w * f};
+                uint32_t w[4];
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    split_half2(v[2 * s], v[2 * s + 4], a[s][0], a[s][1]);
-                    split_half2(v[2 * s + 1], v[2 * s + 5], a[s][2], a[s][3]);
-                    if constexpr (R == 8) {
-                        if (warp == 0) qs[(b * 2 + s) * 32 + lane] = make_uint4(a[s][0], a[s][1], a[s][2], a[s][3]);
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) qf[b][s][c] = a[s][c];
-                    }
+                for (int c = 0; c < 4; ++c) {
+                    const float other = __shfl_xor_sync(0xffffffffu, v[c], 1);
+                    uint32_t hi, lo;
+                    split_half2(lane & 1 ? other : v[c], lane & 1 ? v[c] : other, hi, lo);
+                    w[c] = lane & 1 ? lo : hi;
                 }
+                if (4 * lane < HD)
+                    qs[((4 * n + lane / 8) * 2 + (lane & 1)) * 32 + pair * 4 + (lane & 7) / 2] = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            if constexpr (R == 8) __syncthreads();
         }
+        __syncthreads();
+        // this lane's pairs: g as the products' operand, 2 i and 2 i + 1 in their results
+        const int gpos = seg.pos0 + (seg.pr0 + min(g, seg.npairs - 1)) / G;
+        // the warp's tiles full0 .. full0 + nfull - 1 have no masked position
+        int full0 = 0, nfull = 0;
+        if (seg.all_hi >= AT_TILE - 1) {
+            const int a = (seg.all_lo + AT_TILE - 1) / AT_TILE - seg.t0, b = (seg.all_hi - AT_TILE + 1) / AT_TILE - seg.t0;
+            full0 = max(0, a + S::WARPS - 1) / S::WARPS;
+            nfull = b < 0 ? 0 : max(0, b / S::WARPS + 1 - full0);
+        }
+        const float sfac[2] = {qfac[2 * i], qfac[2 * i + 1]};   // score = sfac * (sum of the products)
 
-        float o[R][4][4];
+        float o[R][2][4];   // (b, t): dims 32 b + 4 g + 2 t (0, 1) and + 1 (2, 3) of pairs 2 i (0, 2) and 2 i + 1 (1, 3)
 #pragma unroll
         for (int b = 0; b < R; ++b)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) o[b][j][c] = 0.0f;
-        float m = -INFINITY;
+                for (int c = 0; c < 4; ++c) o[b][t][c] = 0.0f;
+        // O of the tiles before the last few (see AT_FLUSH), in shared memory: a lane's own values
+        bool kept = false;
+        auto keep = [&](float (&k)[2]) {   // sums = sums * k (+ o, which starts again)
+            float4* sm = reinterpret_cast<float4*>(mine);
+#pragma unroll
+            for (int b = 0; b < R; ++b)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    float4 v = kept ? sm[(2 * b + t) * 32 + lane] : make_float4(0, 0, 0, 0);
+                    v.x = v.x * k[0] + o[b][t][0]; v.y = v.y * k[1] + o[b][t][1];
+                    v.z = v.z * k[0] + o[b][t][2]; v.w = v.w * k[1] + o[b][t][3];
+                    sm[(2 * b + t) * 32 + lane] = v;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) o[b][t][c] = 0.0f;
+                }
+            kept = true;
+        };
+        auto rescale = [&](float (&k)[2]) {
+#pragma unroll
+            for (int b = 0; b < R; ++b)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) o[b][t][c] *= k[c & 1];
+            if (kept) keep(k);
+        };
+        float m[2] = {-INFINITY, -INFINITY};
         float2 l2 = make_float2(0.0f, 0.0f);
         AtScale sv(1);
 
-        for (int k = 0; k < nt; ++k) {
-            const uint32_t n = it + k, slot = n % S::STAGES;
-            if (!mbar_wait_bounded(&bars[slot], (n / S::STAGES) & 1, kv.err, BREW_DEVERR_TIMEOUT_FULL)) {
+        for (int k = 0; k < seg.nt; ++k) {
+            const uint32_t slot = nth % S::STAGES;
+            if (!mbar_wait_bounded(&bars[slot], nth / S::STAGES & 1, kv.err, BREW_DEVERR_TIMEOUT_FULL)) {
                 s_fail = 1;   // recorded; the CTA stops after this item
                 break;
             }
             const uint8_t* tile = ring + slot * S::TILE_BYTES;
-            const int tpos = (t0 + warp + k * AT_WARPS) * AT_TILE;
-            const bool full = tpos >= kall_lo && tpos + AT_TILE - 1 <= kall_hi;   // no position is masked
-
-            // ---- scores of positions 8 u + 2 i + e (u = 0 .. 3), log2 units
-            float2 s[4];
+            // ---- scores (log2 units) of positions 16 gr + g (0, 1) and + 8 (2, 3), pairs 2 i and 2 i + 1
+            float s[2][4];
+            {
+                uint32_t kw[2][2][R];
+                __half d[2][2][R];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) s[u] = make_float2(0.0f, 0.0f);
-            if constexpr (R == 8) {
-                uint32_t kw[4][8];
-                uint32_t sc[4][8];
+                for (int gr = 0; gr < 2; ++gr)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    load_words<R>(kw[u], tile + (u >> 1) * kv_group_bytes(R), u & 1, lane);
-                    load_scales<R>(sc[u], tile + (u >> 1) * kv_group_bytes(R) + 512 * R, u & 1, i);
-                }
+                    for (int h = 0; h < 2; ++h) {
+                        load_words<R>(kw[gr][h], tile + gr * kv_group_bytes(R), h, lane);
+                        load_kscales<R>(d[gr][h], tile + gr * kv_group_bytes(R) + 512 * R, g + 8 * h);
+                        s[gr][2 * h] = s[gr][2 * h + 1] = 0.0f;
+                    }
 #pragma unroll
                 for (int b = 0; b < R; ++b) {
-                    uint32_t a[2][4];
+                    const uint4 qh = qs[2 * b * 32 + lane], ql = qs[(2 * b + 1) * 32 + lane];
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const uint4 v = qs[(b * 2 + t) * 32 + lane];
-                        a[t][0] = v.x; a[t][1] = v.y; a[t][2] = v.z; a[t][3] = v.w;
-                    }
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        uint32_t x[4];
-                        unpack(x, kw[u][b], base);
-                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        mma_f16(c, a[0], x[0], x[1], c);
-                        mma_f16(c, a[1], x[2], x[3], c);
-                        s[u] = fma2(half2_bits(sc[u][b]), add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), s[u]);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    uint32_t kw[R], sc[R];
-                    load_words<R>(kw, tile + (u >> 1) * kv_group_bytes(R), u & 1, lane);
-                    load_scales<R>(sc, tile + (u >> 1) * kv_group_bytes(R) + 512 * R, u & 1, i);
-#pragma unroll
-                    for (int b = 0; b < R; ++b) {
-                        uint32_t x[4];
-                        unpack(x, kw[b], base);
-                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        mma_f16(c, qf[b][0], x[0], x[1], c);
-                        mma_f16(c, qf[b][1], x[2], x[3], c);
-                        s[u] = fma2(half2_bits(sc[b]), add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), s[u]);
+                    for (int gr = 0; gr < 2; ++gr) {
+                        uint32_t x0[4], x1[4];
+                        unpack(x0, kw[gr][0][b], base);
+                        unpack(x1, kw[gr][1][b], base);
+                        const uint32_t a0[4] = {x0[0], x1[0], x0[1], x1[1]}, a1[4] = {x0[2], x1[2], x0[3], x1[3]};
+                        float c[4];
+                        mma_f16_new(c, a0, ql.x, ql.y);
+                        mma_f16(c, a1, ql.z, ql.w, c);
+                        mma_f16(c, a0, qh.x, qh.y, c);
+                        mma_f16(c, a1, qh.z, qh.w, c);
+                        const float f0 = __half2float(d[gr][0][b]), f1 = __half2float(d[gr][1][b]);
+                        s[gr][0] = fmaf(f0, c[0], s[gr][0]);
+                        s[gr][1] = fmaf(f0, c[1], s[gr][1]);
+                        s[gr][2] = fmaf(f1, c[2], s[gr][2]);
+                        s[gr][3] = fmaf(f1, c[3], s[gr][3]);
                     }
                 }
             }
-            float mx = -INFINITY;
+            uint32_t vsc[4][R];   // V's scales of positions 8 u + 2 i, + 1
 #pragma unroll
-            for (int u = 0; u < 4; ++u) s[u] = make_float2(s[u].x * sfac, s[u].y * sfac);
-            uint32_t dead = 0;   // bit 2 u + e: masked for this lane's pair
-            if (!full) {
+            for (int u4 = 0; u4 < 4; ++u4)
+                load_scales<R>(vsc[u4], tile + (u4 >> 1) * kv_group_bytes(R) + 544 * R, u4 & 1, i);
+            if ((uint32_t)(k - full0) >= (uint32_t)nfull) {   // some position is masked
+                const int tpos = (seg.t0 + k * S::WARPS) * AT_TILE;
+                int qpos[2], qlo[2];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int pos = tpos + 8 * u + 2 * i;
-                    if (pos > qpos || pos < qlo) {
-                        dead |= 1u << (2 * u);
-                        s[u].x = -INFINITY;
+                for (int c = 0; c < 2; ++c) {
+                    qpos[c] = __shfl_sync(0xffffffffu, gpos, 8 * i + 4 * c);
+                    qlo[c] = p.window > 0 ? qpos[c] - p.window + 1 : 0;
+                }
+#pragma unroll
+                for (int gr = 0; gr < 2; ++gr)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int pos = tpos + 16 * gr + 4 * (c & 2) + g;
+                        if (pos > qpos[c & 1] || pos < qlo[c & 1]) s[gr][c] = -INFINITY;
                     }
-                    if (pos + 1 > qpos || pos + 1 < qlo) {
-                        dead |= 2u << (2 * u);
-                        s[u].y = -INFINITY;
-                    }
+                // what lies behind a mask may be anything: no NaN of it gets into a product
+                const int glo = p.window > 0 ? gpos - p.window + 1 : 0;
+#pragma unroll
+                for (int u4 = 0; u4 < 4; ++u4) {
+                    const int pos = tpos + 8 * u4 + 2 * i;
+                    const uint32_t live = (pos > gpos || pos < glo ? 0u : 0xFFFFu) |
+                                          (pos + 1 > gpos || pos + 1 < glo ? 0u : 0xFFFF0000u);
+#pragma unroll
+                    for (int b = 0; b < R; ++b) vsc[u4][b] &= live;
                 }
             }
+            float mx[2];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) mx = fmaxf(mx, fmaxf(s[u].x, s[u].y));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            if (__any_sync(0xffffffffu, mx > m + AT_LAZY)) {
-                const float mn = mx > m + AT_LAZY ? mx : m;
-                const float corr = mn == m ? 1.0f : ex2(m - mn);   // m = -inf: 0
-                m = mn;
-                l2 = make_float2(l2.x * corr, l2.y * corr);
+            for (int c = 0; c < 2; ++c) mx[c] = fmaxf(fmaxf(s[0][c], s[0][c + 2]), fmaxf(s[1][c], s[1][c + 2])) * sfac[c];
+            if (__any_sync(0xffffffffu, mx[0] > m[0] + AT_LAZY || mx[1] > m[1] + AT_LAZY)) {
+                float corr[2];
 #pragma unroll
-                for (int b = 0; b < R; ++b)
+                for (int c = 0; c < 2; ++c) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) o[b][j][c] *= corr;
+                    for (int w = 4; w < 32; w <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], w));
+                    const float mn = mx[c] > m[c] + AT_LAZY ? mx[c] : m[c];
+                    corr[c] = mn == m[c] ? 1.0f : ex2(m[c] - mn);   // m = -inf: 0
+                    m[c] = mn;
+                }
+                l2 = make_float2(l2.x * corr[0], l2.y * corr[1]);
+                rescale(corr);
             }
-            const float mref = m == -INFINITY ? 0.0f : m;
+            const float mref[2] = {m[0] == -INFINITY ? 0.0f : AT_PLOG2 - m[0], m[1] == -INFINITY ? 0.0f : AT_PLOG2 - m[1]};
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                s[u].x = ex2(s[u].x - mref);
-                s[u].y = ex2(s[u].y - mref);
-                l2 = add2(l2, s[u]);
+            for (int gr = 0; gr < 2; ++gr) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[gr][c] = ex2(fmaf(s[gr][c], sfac[c & 1], mref[c & 1]));
+                l2 = add2(l2, make_float2(s[gr][0], s[gr][1]));
+                l2 = add2(l2, make_float2(s[gr][2], s[gr][3]));
             }
 
             // ---- O += (p d_V) (c - 8), a group of 16 positions at a time
-            uint32_t vsc[4][R];
             uint32_t dm = 0;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                load_scales<R>(vsc[u], tile + (u >> 1) * kv_group_bytes(R) + 544 * R, u & 1, i);
-                if (!full) {   // what lies behind a mask may be anything: no NaN of it gets into a product
-                    const uint32_t d2 = dead >> (2 * u);
-                    const uint32_t keep = (d2 & 1 ? 0u : 0xFFFFu) | (d2 & 2 ? 0u : 0xFFFF0000u);
+            for (int u4 = 0; u4 < 4; ++u4)
 #pragma unroll
-                    for (int b = 0; b < R; ++b) vsc[u][b] &= keep;
-                }
-#pragma unroll
-                for (int b = 0; b < R; ++b) dm = maxabs_h2(dm, vsc[u][b]);
-            }
+                for (int b = 0; b < R; ++b) dm = maxabs_h2(dm, vsc[u4][b]);
             {
                 const uint32_t top = max(dm & 0x7FFFu, dm >> 16 & 0x7FFFu) >> 10;   // fp16's exponent field
                 if (__any_sync(0xffffffffu, top >= sv.ve)) {
                     const AtScale next(__reduce_max_sync(0xffffffffu, top) + 1);
-                    const float corr = next.total * (1.0f / sv.total);
+                    float corr[2];
+                    corr[0] = corr[1] = next.total * (1.0f / sv.total);
                     sv = next;
-#pragma unroll
-                    for (int b = 0; b < R; ++b)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) o[b][j][c] *= corr;
+                    rescale(corr);
                 }
                 if (sv.dmul != 0x3C003C00u) {
 #pragma unroll
-                    for (int u = 0; u < 4; ++u)
+                    for (int u4 = 0; u4 < 4; ++u4)
 #pragma unroll
-                        for (int b = 0; b < R; ++b) vsc[u][b] = mul_h2(vsc[u][b], sv.dmul);
+                        for (int b = 0; b < R; ++b) vsc[u4][b] = mul_h2(vsc[u4][b], sv.dmul);
                 }
             }
 #pragma unroll
             for (int gr = 0; gr < 2; ++gr) {
-                const uint8_t* grp = tile + gr * kv_group_bytes(R);
                 uint32_t vw[2][R], ph[2], pl[2];
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    load_words<R>(vw[c], grp + 256 * R, c, lane);
-                    split_half2(s[2 * gr + c].x * AT_PSCALE, s[2 * gr + c].y * AT_PSCALE, ph[c], pl[c]);
+                    load_words<R>(vw[c], tile + gr * kv_group_bytes(R) + 256 * R, c, lane);
+                    // p of (position g, pairs 2 i and + 1), transposed to (pair g, positions 2 i and + 1)
+                    split_half2(s[gr][2 * c], s[gr][2 * c + 1], ph[c], pl[c]);
+                    ph[c] = transpose8(ph[c]);
+                    pl[c] = transpose8(pl[c]);
                 }
 #pragma unroll
                 for (int b = 0; b < R; ++b) {
                     // p d as two fp16 numbers: the rounded ph d, and its exact rest plus pl d
-                    uint32_t a[4];
-                    a[0] = mul_h2(ph[0], vsc[2 * gr][b]);
-                    a[1] = fma_h2(pl[0], vsc[2 * gr][b], fma_h2(ph[0], vsc[2 * gr][b], neg_h2(a[0])));
-                    a[2] = mul_h2(ph[1], vsc[2 * gr + 1][b]);
-                    a[3] = fma_h2(pl[1], vsc[2 * gr + 1][b], fma_h2(ph[1], vsc[2 * gr + 1][b], neg_h2(a[2])));
+                    const uint32_t v0 = vsc[2 * gr][b], v1 = vsc[2 * gr + 1][b];
+                    const uint32_t h0 = mul_h2(ph[0], v0), h1 = mul_h2(ph[1], v1);
+                    const uint32_t r0 = fma_h2(pl[0], v0, fma_h2(ph[0], v0, neg_h2(h0)));
+                    const uint32_t r1 = fma_h2(pl[1], v1, fma_h2(ph[1], v1, neg_h2(h1)));
                     uint32_t x0[4], x1[4];
                     unpack(x0, vw[0][b], base);
                     unpack(x1, vw[1][b], base);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_f16(o[b][j], a, x0[j], x1[j], o[b][j]);
+                    for (int t = 0; t < 2; ++t) {
+                        const uint32_t a[4] = {x0[2 * t], x0[2 * t + 1], x1[2 * t], x1[2 * t + 1]};
+                        mma_f16(o[b][t], a, r0, r1, o[b][t]);
+                        mma_f16(o[b][t], a, h0, h1, o[b][t]);
+                    }
                 }
             }
             __syncwarp();   // every lane has read the stage
-            if (((k + S::STAGES) & 31) == 0 && k + S::STAGES < nt) lookup(k + S::STAGES);
-            if (k + S::STAGES < nt) issue(k + S::STAGES);
+            if (k + S::STAGES < seg.nt) {
+                if (((k + S::STAGES) & 31) == 0) lookup(seg, k + S::STAGES);
+                issue(k + S::STAGES, nth);
+            }
+            ++nth;
+            if ((k & (AT_FLUSH - 1)) == AT_FLUSH - 1) {
+                float one[2] = {1.0f, 1.0f};
+                keep(one);
+            }
         }
-        it += nt;
 
-        // ---- the warps' results meet in shared memory (each in its own ring)
-        float l = l2.x + l2.y;
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        float* mine = reinterpret_cast<float*>(ring);   // [pairs][HD], then [pairs][2]
+        // ---- the next item's first tiles, then this one's result
+        const int64_t at = u;
+        u += seg.ub - seg.ua;
+        if (tid == 0) s_done = seg;
+        __syncwarp();
+        const bool more = u < u_end;
+        if (more) {
+            locate(u, seg);
+            __syncwarp();
+            fill(seg);
+        }
+        float l[2] = {l2.x, l2.y};
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], w);
         {
+            if (kept) {
+                const float4* sm = reinterpret_cast<const float4*>(mine);
+#pragma unroll
+                for (int b = 0; b < R; ++b)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const float4 v = sm[(2 * b + t) * 32 + lane];
+                        o[b][t][0] += v.x; o[b][t][1] += v.y; o[b][t][2] += v.z; o[b][t][3] += v.w;
+                    }
+                __syncwarp();
+            }
             const float un = 1.0f / sv.total;
 #pragma unroll
-            for (int b = 0; b < R; ++b)
+            for (int c = 0; c < 2; ++c) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const float4 x = make_float4((o[b][0][c] + o[b][0][c + 2]) * un,
-                                                 (o[b][1][c] + o[b][1][c + 2]) * un,
-                                                 (o[b][2][c] + o[b][2][c + 2]) * un,
-                                                 (o[b][3][c] + o[b][3][c + 2]) * un);
-                    *reinterpret_cast<float4*>(mine + g * HD + 32 * b + 8 * i + 4 * c) = x;
+                for (int b = 0; b < R; ++b)
+                    *reinterpret_cast<float4*>(mine + (2 * i + c) * S::PITCH + 32 * b + 4 * g) =
+                        make_float4(o[b][0][c] * un, o[b][0][c + 2] * un, o[b][1][c] * un, o[b][1][c + 2] * un);
+                if (g == 0) {
+                    mine[AT_PAIRS * S::PITCH + 2 * (2 * i + c)] = m[c];
+                    mine[AT_PAIRS * S::PITCH + 2 * (2 * i + c) + 1] = l[c];
                 }
-            if (i == 0) {
-                mine[AT_PAIRS * HD + 2 * g] = m;
-                mine[AT_PAIRS * HD + 2 * g + 1] = l;
             }
         }
         __syncthreads();
-        const bool whole = ua == 0 && ub == sp.units;
-        float* slot = parts + (int64_t)(cta * 2 + (u == u_begin ? 0 : 1)) * PART;
-        for (int x = tid; x < npairs * (HD / 4); x += AT_THREADS) {
+        const bool whole = done.ua == 0 && done.ub == done.units;
+        float* slot = parts + (int64_t)(cta * 2 + (at == u_begin ? 0 : 1)) * at_part_floats(HD);
+        for (int x = tid; x < done.npairs * (HD / 4); x += S::THREADS) {
             const int r = x / (HD / 4), d = x % (HD / 4) * 4;
-            float M = -INFINITY, L = 0.0f, wt[AT_WARPS];
+            const float* res = reinterpret_cast<const float*>(smem + S::WARPS * S::RING);
+            constexpr int ML = AT_PAIRS * S::PITCH, WARP = S::SUMS / 4;
+            float M = -INFINITY, L = 0.0f;
 #pragma unroll
-            for (int w = 0; w < AT_WARPS; ++w)
-                M = fmaxf(M, reinterpret_cast<float*>(smem + w * S::RING)[AT_PAIRS * HD + 2 * r]);
+            for (int w = 0; w < S::WARPS; ++w) M = fmaxf(M, res[w * WARP + ML + 2 * r]);
             float4 a = make_float4(0, 0, 0, 0);
 #pragma unroll
-            for (int w = 0; w < AT_WARPS; ++w) {
-                const float* sw = reinterpret_cast<float*>(smem + w * S::RING);
-                const float mw = sw[AT_PAIRS * HD + 2 * r];
-                wt[w] = mw == -INFINITY ? 0.0f : ex2(mw - M);
-                L += wt[w] * sw[AT_PAIRS * HD + 2 * r + 1];
-                const float4 v = *reinterpret_cast<const float4*>(sw + r * HD + d);
-                a.x += wt[w] * v.x; a.y += wt[w] * v.y; a.z += wt[w] * v.z; a.w += wt[w] * v.w;
+            for (int w = 0; w < S::WARPS; ++w) {
+                const float mw = res[w * WARP + ML + 2 * r];
+                const float wt = mw == -INFINITY ? 0.0f : ex2(mw - M);
+                L += wt * res[w * WARP + ML + 2 * r + 1];
+                const float4 v = *reinterpret_cast<const float4*>(res + w * WARP + r * S::PITCH + d);
+                a.x += wt * v.x; a.y += wt * v.y; a.z += wt * v.z; a.w += wt * v.w;
             }
             if (whole) {
-                const int pr = pr0 + r, j = pr / G;
+                const int pr = done.pr0 + r, j = pr / G;
                 const float inv = 1.0f / L;
-                *reinterpret_cast<float4*>(p.out + (int64_t)(e.row0 + j) * p.ldo + (int64_t)(hk * G + pr - j * G) * HD + d) =
+                *reinterpret_cast<float4*>(p.out + (int64_t)(done.row0 + j) * p.ldo + (int64_t)(done.hk * G + pr - j * G) * HD + d) =
                     make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
             } else {
                 __stcg(reinterpret_cast<float4*>(slot + r * HD + d), a);
@@ -612,57 +722,74 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<R>::CTAS_PER_SM)
             }
         }
         if (!whole) {
-            // the item's CTAs; the last one to arrive joins their parts
-            const int64_t v0 = prefix[lo] + (int64_t)item * sp.units;
-            const int c0 = cta_of(v0, U, C), c1 = cta_of(v0 + sp.units - 1, U, C), np = c1 - c0 + 1;
-            const bool c0_first = U * c0 / C >= v0;   // the item is the first of CTA c0's run
-            __syncthreads();
-            if (tid == 0) {
-                __threadfence();
-                s_last = atomicAdd(&counters[c0], 1) == np - 1;
-            }
-            __syncthreads();
-            if (s_last) {
-                __threadfence();
-                auto part = [&](int c) { return parts + (int64_t)((c0 + c) * 2 + (c == 0 && !c0_first)) * PART; };
-                // weights [part][pair] into shared memory
-                float* wt = reinterpret_cast<float*>(smem);
-                float* tot = wt + AT_MAX_CTAS * AT_PAIRS;   // [pair] sum, then the warps' sums [warp][pairs][HD]
-                for (int r = warp; r < npairs; r += AT_WARPS) {
-                    float M = -INFINITY, L = 0.0f;
-                    for (int c = lane; c < np; c += 32) M = fmaxf(M, __ldcg(part(c) + AT_PAIRS * HD + 2 * r));
-                    M = warp_max(M);
-                    for (int c = lane; c < np; c += 32) {
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(part(c) + AT_PAIRS * HD + 2 * r));
-                        const float w = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
-                        wt[c * AT_PAIRS + r] = w;
-                        L += w * ml.y;
-                    }
-                    L = warp_sum(L);
-                    if (lane == 0) tot[r] = 1.0f / L;
-                }
-                __syncthreads();
-                for (int x = tid; x < npairs * (HD / 4); x += AT_THREADS) {
-                    const int r = x / (HD / 4), d = x % (HD / 4) * 4;
-                    float4 a = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-                    for (int c = 0; c < np; ++c) {
-                        const float w = wt[c * AT_PAIRS + r];
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(part(c) + r * HD + d));
-                        a.x += w * v.x; a.y += w * v.y; a.z += w * v.z; a.w += w * v.w;
-                    }
-                    const int pr = pr0 + r, j = pr / G;
-                    const float inv = tot[r];
-                    *reinterpret_cast<float4*>(p.out + (int64_t)(e.row0 + j) * p.ldo + (int64_t)(hk * G + pr - j * G) * HD + d) =
-                        make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-                }
-                if (tid == 0) counters[c0] = 0;
-            }
+            if (at == u_begin) split_first = true;
+            else split_last = true;
+            if (tid == 0) s_ends[at != u_begin] = done;
         }
-        fence_proxy_async();   // these plain accesses come before the next item's bulk copies
-        __syncthreads();
+        __syncthreads();   // the results are read, the next q may be written
         if (s_fail) return;
-        u += ub - ua;
+        if (!more) break;
+    }
+
+    // ---- shared items: the last of an item's CTAs to get here joins its parts
+    if (!split_first && !split_last) return;
+    int np[2] = {0, 0}, c0[2] = {0, 0};
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        if (!(x == 0 ? split_first : split_last)) continue;
+        c0[x] = cta_of(s_ends[x].item0, U, C);
+        np[x] = cta_of(s_ends[x].item0 + s_ends[x].units - 1, U, C) - c0[x] + 1;
+    }
+    if (tid == 0) {
+        __threadfence();
+#pragma unroll
+        for (int x = 0; x < 2; ++x) s_join[x] = np[x] > 0 && atomicAdd(&counters[c0[x]], 1) == np[x] - 1;
+        __threadfence();
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        if (!s_join[x]) continue;
+        const AtSeg& e = s_ends[x];
+        const bool first = U * c0[x] / C >= e.item0;   // the item is the first of CTA c0's run
+        auto part = [&](int c) { return parts + (int64_t)((c0[x] + c) * 2 + (c == 0 && !first)) * at_part_floats(HD); };
+        for (int r = warp; r < e.npairs; r += S::WARPS) {   // a warp for a pair
+            float* wt = reinterpret_cast<float*>(ring);
+            const float* ml = parts + AT_PAIRS * HD + 2 * r;
+            float M = -INFINITY, L = 0.0f;
+            for (int c = lane; c < np[x]; c += 32) {
+                wt[c] = __ldcg(ml + (part(c) - parts));
+                M = fmaxf(M, wt[c]);
+            }
+            M = warp_max(M);
+            for (int c = lane; c < np[x]; c += 32) {
+                wt[c] = wt[c] == -INFINITY ? 0.0f : ex2(wt[c] - M);
+                L += wt[c] * __ldcg(ml + (part(c) - parts) + 1);
+            }
+            L = warp_sum(L);
+            __syncwarp();
+            const int pr = e.pr0 + r, j = pr / G;
+            float* dst = p.out + (int64_t)(e.row0 + j) * p.ldo + (int64_t)(e.hk * G + pr - j * G) * HD;
+            const float inv = 1.0f / L;
+            for (int d = 4 * lane; d < HD; d += 128) {
+                float4 a = make_float4(0, 0, 0, 0);
+                constexpr int AHEAD = 16;   // loads in flight
+                for (int c = 0; c < np[x]; c += AHEAD) {
+                    float4 v[AHEAD];
+#pragma unroll
+                    for (int y = 0; y < AHEAD; ++y)
+                        v[y] = __ldcg(reinterpret_cast<const float4*>(part(min(c + y, np[x] - 1)) + r * HD + d));
+#pragma unroll
+                    for (int y = 0; y < AHEAD; ++y) {
+                        const float w = c + y < np[x] ? wt[c + y] : 0.0f;
+                        a.x += w * v[y].x; a.y += w * v[y].y; a.z += w * v[y].z; a.w += w * v[y].w;
+                    }
+                }
+                *reinterpret_cast<float4*>(dst + d) = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+            }
+            __syncwarp();   // wt is the next pair's
+        }
+        if (tid == 0) counters[c0[x]] = 0;
     }
 }
 
@@ -671,15 +798,15 @@ int attend_r(const KvAttendParams& p, cudaStream_t s) {
     using S = AtShape<R>;
     static std::mutex mu;
     static unsigned long long done = 0;
-    const int smem = S::PREFIX + 8 * (p.rows.n_seqs + 1);
+    constexpr int smem = S::PREFIX + 8 * S::THREADS;
     {
         std::lock_guard<std::mutex> lk(mu);
-        BREW_CUDA(smem_attr_per_device((const void*)kv_attend_kernel<R>, S::PREFIX + 8 * (KV_MAX_SEQS + 1), &done));
+        BREW_CUDA(smem_attr_per_device((const void*)kv_attend_kernel<R>, smem, &done));
     }
     const int ctas = std::min(AT_MAX_CTAS, S::CTAS_PER_SM * num_sms());
     KvAttendParams q = p;
     q.code_base = 0x64006400u;
-    kv_attend_kernel<R><<<ctas, AT_THREADS, smem, s>>>(q);
+    kv_attend_kernel<R><<<ctas, S::THREADS, smem, s>>>(q);
     BREW_CUDA(cudaGetLastError());
     count_launch();
     return BREW_OK;
@@ -688,7 +815,7 @@ int attend_r(const KvAttendParams& p, cudaStream_t s) {
 }  // namespace
 
 int64_t kv_attend_workspace(int head_size) {
-    return 4096 + (int64_t)AT_MAX_CTAS * 2 * AT_PAIRS * (head_size + 2) * 4;
+    return AT_COUNTER_BYTES + (int64_t)AT_MAX_CTAS * 2 * at_part_floats(head_size) * 4;
 }
 
 int kv_attend_launch(int hd, const KvAttendParams& p, cudaStream_t s) {

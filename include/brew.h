@@ -481,7 +481,7 @@ BREW_API int brew_kv_read_dev(brew_kv kv, int32_t layer, float* k_out, float* v_
  * 0); scale 0 means 1 / sqrt(head_size).  out may not overlap q.  `workspace`:
  * brew_kv_workspace_bytes(kv) device bytes on a 256-byte boundary,
  * zero-filled once before its first use (each call leaves it ready for the
- * next).  Calls and captured graphs that may run at the same time need a
+ * next, unless brew_kv_check reports BREW_ERR_TIMEOUT).  Calls and captured graphs that may run at the same time need a
  * workspace each. */
 BREW_API int64_t brew_kv_workspace_bytes(brew_kv kv);
 BREW_API int brew_kv_attend_dev(brew_kv kv, int32_t layer, float* out, int64_t ldo, const float* q, int64_t ldq,

@@ -15,14 +15,18 @@ static int fails = 0;
 
 template <int R>
 void layout() {
-    std::set<int> words, scales;
+    std::set<int> words, kscales, vscales;
     for (int u = 0; u < 2; ++u)
         for (int b = 0; b < R; ++b)
             for (int lane = 0; lane < 32; ++lane) words.insert(kv_word(R, u, b, lane));
     EXPECT((int)words.size() == 64 * R && *words.begin() == 0 && *words.rbegin() == 64 * R - 1);
     for (int p = 0; p < 16; ++p)
-        for (int b = 0; b < R; ++b) scales.insert(kv_scale(R, p, b));
-    EXPECT((int)scales.size() == 16 * R && *scales.begin() == 0 && *scales.rbegin() == 16 * R - 1);
+        for (int b = 0; b < R; ++b) {
+            kscales.insert(kv_kscale(R, p, b));
+            vscales.insert(kv_vscale(R, p, b));
+        }
+    for (const std::set<int>& s : {kscales, vscales})
+        EXPECT((int)s.size() == 16 * R && *s.begin() == 0 && *s.rbegin() == 16 * R - 1);
     EXPECT(kv_group_bytes(R) == 2 * 256 * R + 2 * 32 * R && kv_group_bytes(R) % 16 == 0);
     for (int shift = 4; shift <= 7; ++shift) {
         const int n_pages = 7, n_kv = 3, max_pages = 3, page = 1 << shift;
