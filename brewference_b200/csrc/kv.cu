@@ -54,145 +54,184 @@ int set_pages(brew_kv_s* kv, int seq, size_t first, size_t end, int tokens, cuda
 }
 
 // ---- append -------------------------------------------------------------
-// One CTA per row.  The row's angles are computed once, in 64 bits (a
-// position of 10^5 leaves 32 bits no digit of the angle), and shared by all
-// heads; norm and rotation run in 64 bits too and are rounded once, because
-// the 4-bit code of a value next to a rounding border depends on its last
-// bit.  A vector (one head of q, k or v) is held by LPV lanes, 4 dims each
-// (twice for heads of 256); a block of 32 values is 8 lanes.
+// The 4-bit code of a value next to a rounding border depends on its last
+// bit (and a position of 10^5 leaves 32 bits no digit of the angle), so
+// angles, norm and rotation run in 64 bits and are rounded once.
+//
+// A CTA takes up to AP_ROWS rows of an entry; their sines and the norm's
+// weights are made once and shared by all heads.  A lane holds 16 dims of a
+// vector (a head of q, k or v) in two pieces of 8, the second half a head
+// after the first where blocks of 32 allow it (heads of 64, 128, 256): then
+// the pairs of either rotation are the lane's own, a piece is a word of K's
+// codes, and no value is converted twice.  (4 dims a lane, partners loaded
+// and converted again: 102 us for 5194 rows of 16 + 16 heads of 128; the same
+// in pairs of fp32 numbers instead of 64 bits: 69 us.)
 constexpr int AP_THREADS = 256;
+constexpr int AP_ROWS = 4;
 
-template <int R>
+template <int R, bool NORM, int ROPE>
 __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(const __grid_constant__ KvAppendParams p) {
-    constexpr int HD = 32 * R;
-    constexpr int LPV = R == 1 ? 8 : R == 2 ? 16 : 32;   // lanes a vector (R = 3: 24 of them hold values)
-    constexpr int NV = R == 8 ? 2 : 1;                   // float4s a lane
-    constexpr int VPW = 32 / LPV;                        // vectors of a warp
-    __shared__ double cs[HD / 2], sn[HD / 2];
+    constexpr int HD = 32 * R, HALF = HD / 2;
+    constexpr bool OWN = R % 2 == 0;          // pieces half a head apart (else side by side)
+    constexpr int LPV = R == 3 ? 8 : 2 * R;   // lanes a vector (R = 3: 6 of them hold values)
+    constexpr int VPW = 32 / LPV;             // vectors of a warp
+    constexpr int SL = HALF / 8;              // sines lie [i % 8][i / 8]: a step's are side by side over the lanes
+    __shared__ double2 cs[AP_ROWS][HALF];     // cosine, sine
+    __shared__ double wq[NORM ? HD : 1], wk[NORM ? HD : 1];   // [d % 8][d / 8]
     const KvEntry e = kv_entry(p.kv, p.rows, blockIdx.y, threadIdx.x == 0 && blockIdx.x == 0);
-    const int j = blockIdx.x;
-    if (j >= e.rows) return;
-    const int pos = e.pos0 + j;
-    const int64_t row = e.row0 + j;
-    if (p.rope != BREW_KV_ROPE_NONE) {
-        for (int i = threadIdx.x; i < HD / 2; i += AP_THREADS) {
-            const double a = (double)pos * p.rope_scale * exp2(-2.0 * i * p.log2_base_hd);
-            sincos(a, &sn[i], &cs[i]);
+    const int j0 = blockIdx.x * AP_ROWS, nr = min(AP_ROWS, e.rows - j0);
+    if (nr <= 0) return;
+    auto wat = [](int d) { return d % 8 * (HD / 8) + d / 8; };
+    auto sat = [](int i) { return i % 8 * SL + i / 8; };
+    if (ROPE != BREW_KV_ROPE_NONE) {
+        for (int x = threadIdx.x; x < nr * HALF; x += AP_THREADS) {
+            const int r = x / HALF, i = x % HALF;
+            double c, s;
+            sincos((double)(e.pos0 + j0 + r) * p.rope_scale * exp2(-2.0 * i * p.log2_base_hd), &s, &c);
+            cs[r][sat(i)] = make_double2(c, s);
         }
-        __syncthreads();
     }
+    if (NORM) {
+        for (int d = threadIdx.x; d < HD; d += AP_THREADS) {
+            wq[wat(d)] = p.qnorm ? (double)p.qnorm[d] : 1.0;
+            wk[wat(d)] = p.knorm ? (double)p.knorm[d] : 1.0;
+        }
+    }
+    if (NORM || ROPE != BREW_KV_ROPE_NONE) __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int l = lane % LPV;
-    const bool act = R != 3 || l < 24;
+    const int dim[2] = {OWN ? 8 * l : 16 * l, OWN ? 8 * l + HALF : 16 * l + 8};   // the pieces
+    const bool act = R != 3 || l < 6;
     const int hq = p.q ? p.kv.n_heads : 0, hk = p.kv.n_kv;
     const int nvec = hq + 2 * hk;
-    for (int v0 = warp * VPW; v0 < nvec; v0 += AP_THREADS / 32 * VPW) {   // uniform over the warp
-        const int v = v0 + lane / LPV;
-        const bool on = act && v < nvec;
-        const bool isq = v < hq, isk = !isq && v < hq + hk;
-        const int head = isq ? v : isk ? v - hq : v - hq - hk;
-        const float* src = (isq ? p.q + row * p.ldq : (isk ? p.k : p.v) + row * p.ldkv) + (int64_t)head * HD;
-        const float* w = isq ? p.qnorm : isk ? p.knorm : nullptr;
-        float x[NV][4];
+    for (int r = 0; r < nr; ++r) {
+        const int pos = e.pos0 + j0 + r;
+        const int64_t row = (int64_t)e.row0 + j0 + r;
+        const int64_t grp0 = kv_group_at<R>(p.kv, e.seq, pos, 0);   // kv head 0's; the next ones' follow a page's groups apart
+        const int pg = pos & 15, u = pg >> 3;
+        for (int v0 = warp * VPW; v0 < nvec; v0 += AP_THREADS / 32 * VPW) {   // uniform over the warp
+            const int v = v0 + lane / LPV;
+            const bool on = act && v < nvec;
+            const bool isq = v < hq, isk = !isq && v < hq + hk;
+            const bool qk = on && (isq || isk);
+            const int head = isq ? v : isk ? v - hq : v - hq - hk;
+            const float* src = (isq ? p.q + row * p.ldq : (isk ? p.k : p.v) + row * p.ldkv) + (int64_t)head * HD;
+            float x[2][8], y[2][8];   // the pieces, and (!OWN) their dims' partners half a head away
 #pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            const float4 t = on ? *reinterpret_cast<const float4*>(src + 128 * n + 4 * l) : make_float4(0, 0, 0, 0);
-            x[n][0] = t.x; x[n][1] = t.y; x[n][2] = t.z; x[n][3] = t.w;
-        }
-        double inv = 1.0;
-        if (p.qnorm || p.knorm) {   // uniform
-            double ss = 0.0;
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int n = 0; n < NV; ++n)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) ss += (double)x[n][c] * (double)x[n][c];
-#pragma unroll
-            for (int o = LPV / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            inv = 1.0 / sqrt(ss / HD + p.eps);
-        }
-        float y[NV][4];
-#pragma unroll
-        for (int n = 0; n < NV; ++n)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) y[n][c] = x[n][c];
-        if (on && (isq || isk) && (w || p.rope != BREW_KV_ROPE_NONE)) {
-#pragma unroll
-            for (int n = 0; n < NV; ++n) {
-                const int d0 = 128 * n + 4 * l;
-                double a[4], b[4] = {0, 0, 0, 0};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) a[c] = w ? (double)x[n][c] * inv * (double)w[d0 + c] : (double)x[n][c];
-                if (p.rope == BREW_KV_ROPE_HALF) {   // pairs (d, d + hd / 2)
-                    const bool lowd = d0 < HD / 2;
-                    const int m0 = lowd ? d0 + HD / 2 : d0 - HD / 2;
-                    const float4 t = *reinterpret_cast<const float4*>(src + m0);
-                    b[0] = t.x; b[1] = t.y; b[2] = t.z; b[3] = t.w;
-                    if (w)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) b[c] = b[c] * inv * (double)w[m0 + c];
-                    const int i0 = lowd ? d0 : m0;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        a[c] = lowd ? a[c] * cs[i0 + c] - b[c] * sn[i0 + c] : b[c] * sn[i0 + c] + a[c] * cs[i0 + c];
-                } else if (p.rope == BREW_KV_ROPE_INTERLEAVED) {   // pairs (2 i, 2 i + 1)
-#pragma unroll
-                    for (int c = 0; c < 4; c += 2) {
-                        const int i = (d0 + c) / 2;
-                        const double r0 = a[c] * cs[i] - a[c + 1] * sn[i], r1 = a[c] * sn[i] + a[c + 1] * cs[i];
-                        a[c] = r0;
-                        a[c + 1] = r1;
+                for (int c = 0; c < 8; c += 4) {
+                    const float4 t = on ? *reinterpret_cast<const float4*>(src + dim[h] + c) : make_float4(0, 0, 0, 0);
+                    x[h][c] = t.x; x[h][c + 1] = t.y; x[h][c + 2] = t.z; x[h][c + 3] = t.w;
+                    if (!OWN && ROPE == BREW_KV_ROPE_HALF) {
+                        const int m = dim[h] < HALF ? dim[h] + HALF : dim[h] - HALF;
+                        const float4 o = qk ? *reinterpret_cast<const float4*>(src + m + c) : make_float4(0, 0, 0, 0);
+                        y[h][c] = o.x; y[h][c + 1] = o.y; y[h][c + 2] = o.z; y[h][c + 3] = o.w;
                     }
                 }
+            double inv = 1.0;
+            if (NORM && v0 < hq + hk) {   // uniform over the warp: the shuffles are every lane's
+                double ss = 0.0;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) y[n][c] = (float)a[c];
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) ss = fma((double)x[h][c], (double)x[h][c], ss);
+#pragma unroll
+                for (int o = LPV / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const bool has = isq ? p.qnorm != nullptr : p.knorm != nullptr;
+                inv = has ? rsqrt(ss * (1.0 / HD) + p.eps) : 1.0;
             }
-        }
-        __syncwarp();   // q_out may be q: every lane has read before one writes
-        if (on && isq) {
-            float* dst = p.q_out + row * p.ldq + (int64_t)head * HD;
+            __syncwarp();   // q_out may be q: every lane has read before one writes
+            if ((NORM || ROPE != BREW_KV_ROPE_NONE) && qk) {
+                const double* w = isq ? wq : wk;
+                // a dim with its norm
+                auto in = [&](float t, int d) { return NORM ? (double)t * inv * w[wat(d)] : (double)t; };
 #pragma unroll
-            for (int n = 0; n < NV; ++n)
-                *reinterpret_cast<float4*>(dst + 128 * n + 4 * l) = make_float4(y[n][0], y[n][1], y[n][2], y[n][3]);
-        }
+                for (int c = 0; c < 8; ++c) {
+                    if (ROPE == BREW_KV_ROPE_HALF && OWN) {   // the pieces are each other's partners
+                        const double2 t = cs[r][c * SL + l];
+                        const double a = in(x[0][c], dim[0] + c), b = in(x[1][c], dim[1] + c);
+                        x[0][c] = (float)(a * t.x - b * t.y);
+                        x[1][c] = (float)(a * t.y + b * t.x);
+                    } else if (ROPE == BREW_KV_ROPE_HALF) {
 #pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            // the block's scale: -1/8 of its first value of largest magnitude
-            uint32_t m = 0;
+                        for (int h = 0; h < 2; ++h) {
+                            const int d = dim[h] + c;
+                            const bool low = d < HALF;
+                            const double2 t = cs[r][sat(low ? d : d - HALF)];
+                            const double a = in(x[h][c], d), b = in(y[h][c], low ? d + HALF : d - HALF);
+                            x[h][c] = (float)(low ? a * t.x - b * t.y : b * t.y + a * t.x);
+                        }
+                    } else if (ROPE == BREW_KV_ROPE_INTERLEAVED) {
+                        if (c % 2) continue;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) m = max(m, __float_as_uint(y[n][c]) & 0x7fffffffu);
-            uint32_t mb = m;
+                        for (int h = 0; h < 2; ++h) {
+                            const double2 t = cs[r][sat((dim[h] + c) / 2)];
+                            const double a = in(x[h][c], dim[h] + c), b = in(x[h][c + 1], dim[h] + c + 1);
+                            x[h][c] = (float)(a * t.x - b * t.y);
+                            x[h][c + 1] = (float)(a * t.y + b * t.x);
+                        }
+                    } else {
 #pragma unroll
-            for (int o = 4; o > 0; o >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, o));
-            float mine = y[n][3];
-#pragma unroll
-            for (int c = 2; c >= 0; --c)
-                if ((__float_as_uint(y[n][c]) & 0x7fffffffu) == mb) mine = y[n][c];
-            const uint32_t has = __ballot_sync(0xffffffffu, m == mb) >> (lane & 24) & 255u;
-            const float top = __shfl_sync(0xffffffffu, mine, (lane & 24) + __ffs(has) - 1);
-            float d = top * -0.125f;
-            // fp16 ends at 65504: larger blocks saturate (a NaN stays one)
-            if (fabsf(d) > 65504.0f) d = copysignf(65504.0f, d);
-            const float id = d == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);
-            uint32_t q = 0;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int t = (int)truncf(__fadd_rn(__fmul_rn(y[n][c], id), 8.5f));
-                q |= (uint32_t)max(0, min(15, t)) << (4 * c);
+                        for (int h = 0; h < 2; ++h) x[h][c] = (float)in(x[h][c], dim[h] + c);
+                    }
+                }
             }
-            const uint32_t next = __shfl_down_sync(0xffffffffu, q, 1);
+            if (on && isq) {
+                float* dst = p.q_out + row * p.ldq + (int64_t)head * HD;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int c = 0; c < 8; c += 4)
+                        *reinterpret_cast<float4*>(dst + dim[h] + c) =
+                            make_float4(x[h][c], x[h][c + 1], x[h][c + 2], x[h][c + 3]);
+            }
+            if (v0 + VPW <= hq) continue;   // a warp of q alone
+            // a block's scale: -1/8 of its first value of largest magnitude, of a piece, then of the block's lanes
+            float top[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                top[h] = x[h][0];
+#pragma unroll
+                for (int c = 1; c < 8; ++c) top[h] = fabsf(x[h][c]) > fabsf(top[h]) || x[h][c] != x[h][c] ? x[h][c] : top[h];
+            }
+            if (!OWN && (fabsf(top[1]) > fabsf(top[0]) || top[1] != top[1])) top[0] = top[1];   // one block
+#pragma unroll
+            for (int h = 0; h < (OWN ? 2 : 1); ++h)
+#pragma unroll
+                for (int o = 1; o < (OWN ? 4 : 2); o <<= 1) {
+                    const float other = __shfl_xor_sync(0xffffffffu, top[h], o);
+                    const bool take = lane & o ? !(fabsf(top[h]) > fabsf(other)) : fabsf(other) > fabsf(top[h]);
+                    if ((take && top[h] == top[h]) || other != other) top[h] = other;
+                }
+            if (!OWN) top[1] = top[0];
             if (!on || isq) continue;
-            uint8_t* grp = kv_group<R>(p.kv, e.seq, pos, head);
-            const int b = 4 * n + l / 8, pg = pos & 15, u = pg >> 3;
-            if (isk) {
-                uint32_t* kq = reinterpret_cast<uint32_t*>(grp);
-                if ((l & 1) == 0) kq[kv_word(R, u, b, (pg & 7) * 4 + (l & 7) / 2)] = q | next << 16;
-            } else {
-                uint16_t* vq = reinterpret_cast<uint16_t*>(grp + 256 * R);
-                vq[2 * kv_word(R, u, b, (l & 7) * 4 + ((pg & 7) >> 1)) + (pg & 1)] = (uint16_t)q;
-            }
-            if ((l & 7) == 0) {
-                uint16_t* sc = reinterpret_cast<uint16_t*>(grp + 512 * R + (isk ? 0 : 32 * R));
-                sc[isk ? kv_kscale(R, pg, b) : kv_vscale(R, pg, b)] = __half_as_ushort(__float2half_rn(d));
+            uint8_t* grp = p.kv.pages + grp0 + ((int64_t)head << (p.kv.page_shift - 4)) * kv_group_bytes(R);
+            uint16_t* sc = reinterpret_cast<uint16_t*>(grp + 512 * R);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float d = top[h] * -0.125f;
+                // fp16 ends at 65504: larger blocks saturate (a NaN stays one)
+                if (fabsf(d) > 65504.0f) d = copysignf(65504.0f, d);
+                const float id = d == 0.0f ? 0.0f : __frcp_rn(d);
+                uint32_t q = 0;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    // 0 .. 15: the integer part, as the last bits of 2^23 + it
+                    const float t = fminf(fmaxf(__fadd_rn(__fmul_rn(x[h][c], id), 8.5f), 0.0f), 15.5f);
+                    q |= (__float_as_uint(__fadd_rd(t, 8388608.0f)) & 15u) << (4 * c);
+                }
+                const int b = dim[h] / 32, i = dim[h] % 32 / 8;
+                const uint16_t dh = __half_as_ushort(__float2half_rn(d));
+                if (isk) {
+                    reinterpret_cast<uint32_t*>(grp)[kv_word(R, u, b, (pg & 7) * 4 + i)] = q;
+                    if (i == 0) sc[kv_kscale(R, pg, b)] = dh;
+                } else {
+                    uint16_t* vq = reinterpret_cast<uint16_t*>(grp + 256 * R);
+                    vq[2 * kv_word(R, u, b, 8 * i + ((pg & 7) >> 1)) + (pg & 1)] = (uint16_t)q;
+                    vq[2 * kv_word(R, u, b, 8 * i + 4 + ((pg & 7) >> 1)) + (pg & 1)] = (uint16_t)(q >> 16);
+                    if (i == 0) sc[16 * R + kv_vscale(R, pg, b)] = dh;
+                }
             }
         }
     }
@@ -200,44 +239,65 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(const __grid_cons
 
 template <int R>
 int append_r(const KvAppendParams& p, cudaStream_t s) {
-    const dim3 grid(p.rows.max_rows, p.rows.n_seqs);
-    kv_append_kernel<R><<<grid, AP_THREADS, 0, s>>>(p);
+    const dim3 grid((p.rows.max_rows + AP_ROWS - 1) / AP_ROWS, p.rows.n_seqs);
+    auto go = [&](auto kernel) { kernel<<<grid, AP_THREADS, 0, s>>>(p); };
+    if (p.qnorm || p.knorm) {
+        if (p.rope == BREW_KV_ROPE_HALF) go(kv_append_kernel<R, true, BREW_KV_ROPE_HALF>);
+        else if (p.rope == BREW_KV_ROPE_INTERLEAVED) go(kv_append_kernel<R, true, BREW_KV_ROPE_INTERLEAVED>);
+        else go(kv_append_kernel<R, true, BREW_KV_ROPE_NONE>);
+    } else {
+        if (p.rope == BREW_KV_ROPE_HALF) go(kv_append_kernel<R, false, BREW_KV_ROPE_HALF>);
+        else if (p.rope == BREW_KV_ROPE_INTERLEAVED) go(kv_append_kernel<R, false, BREW_KV_ROPE_INTERLEAVED>);
+        else go(kv_append_kernel<R, false, BREW_KV_ROPE_NONE>);
+    }
     BREW_CUDA(cudaGetLastError());
     count_launch();
     return BREW_OK;
 }
 
 // ---- read: the values that stored rows stand for --------------------------
-// One thread per 4 dims of a (row, kv head), k and v both.
+// One thread per 8 dims of a (row, kv head), k and v both: a word of k, two
+// halves of words of v.  Bound by the write of 4 bytes a value.
+constexpr int RD_ROWS = 4;
+
+__device__ __forceinline__ void kv_values(float* dst, uint32_t w, float d) {
+    float v[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c)   // 2^23 + code, as bits
+        v[c] = (__uint_as_float((w >> 4 * c & 15u) | 0x4B000000u) - 8388616.0f) * d;
+    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+
 template <int R>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvView kv,
                                                       const __grid_constant__ KvRowsDev rows, float* k_out,
                                                       float* v_out, int64_t ld) {
     const KvEntry e = kv_entry(kv, rows, blockIdx.y, threadIdx.x == 0 && blockIdx.x == 0);
-    const int j = blockIdx.x;
-    if (j >= e.rows) return;
-    const int pos = e.pos0 + j, pg = pos & 15, u = pg >> 3;
-    for (int t = threadIdx.x; t < kv.n_kv * 8 * R; t += 256) {
-        const int hk = t / (8 * R), d4 = t % (8 * R), b = d4 / 8, l = d4 & 7;
+    const int j0 = blockIdx.x * RD_ROWS, nr = min(RD_ROWS, e.rows - j0);
+    const int per = kv.n_kv * 4 * R;   // threads' work of a row
+    for (int x = threadIdx.x; x < nr * per; x += 256) {
+        const int r = x / per, t = x - r * per;
+        const int pos = e.pos0 + j0 + r, pg = pos & 15, u = pg >> 3;
+        const int hk = t / (4 * R), d8 = t % (4 * R), b = d8 / 4, i = d8 & 3;
         const uint8_t* grp = kv_group<R>(kv, e.seq, pos, hk);
-        const int64_t o = (e.row0 + j) * ld + (int64_t)hk * 32 * R + 4 * d4;
-        const uint16_t* kq = reinterpret_cast<const uint16_t*>(grp);
+        const int64_t o = ((int64_t)e.row0 + j0 + r) * ld + (int64_t)hk * 32 * R + 8 * d8;
         const uint16_t* sc = reinterpret_cast<const uint16_t*>(grp + 512 * R);
-        const uint32_t qk = kq[2 * kv_word(R, u, b, (pg & 7) * 4 + l / 2) + (l & 1)];
-        const uint32_t qv = kq[128 * R + 2 * kv_word(R, u, b, l * 4 + ((pg & 7) >> 1)) + (pg & 1)];
+        const uint16_t* vq = reinterpret_cast<const uint16_t*>(grp + 256 * R);
+        const int half = pg & 1, at = (pg & 7) >> 1;
+        const uint32_t wk = reinterpret_cast<const uint32_t*>(grp)[kv_word(R, u, b, (pg & 7) * 4 + i)];
+        const uint32_t wv = vq[2 * kv_word(R, u, b, 8 * i + at) + half] |
+                            (uint32_t)vq[2 * kv_word(R, u, b, 8 * i + 4 + at) + half] << 16;
         const float dk = half_bits_to_float(sc[kv_kscale(R, pg, b)]);
         const float dv = half_bits_to_float(sc[16 * R + kv_vscale(R, pg, b)]);
-        auto val = [](uint32_t q, int c, float d) { return (float)((int)(q >> 4 * c & 15) - 8) * d; };
-        if (k_out)
-            *reinterpret_cast<float4*>(k_out + o) = make_float4(val(qk, 0, dk), val(qk, 1, dk), val(qk, 2, dk), val(qk, 3, dk));
-        if (v_out)
-            *reinterpret_cast<float4*>(v_out + o) = make_float4(val(qv, 0, dv), val(qv, 1, dv), val(qv, 2, dv), val(qv, 3, dv));
+        if (k_out) kv_values(k_out + o, wk, dk);
+        if (v_out) kv_values(v_out + o, wv, dv);
     }
 }
 
 template <int R>
 int read_r(const KvView& kv, const KvRowsDev& rows, float* k, float* v, int64_t ld, cudaStream_t s) {
-    const dim3 grid(rows.max_rows, rows.n_seqs);
+    const dim3 grid((rows.max_rows + RD_ROWS - 1) / RD_ROWS, rows.n_seqs);
     kv_read_kernel<R><<<grid, 256, 0, s>>>(kv, rows, k, v, ld);
     BREW_CUDA(cudaGetLastError());
     count_launch();
