@@ -460,6 +460,23 @@ class DeviceModel:
         matrices on the tcgen05 GEMM)."""
         N.check(N.lib().brew_model_set_prefill(self.handle, int(mode)), "set_prefill")
 
+    def set_kv_cache(self, qtype: int) -> None:
+        """The K/V cache: TYPE_F32 (default) or TYPE_Q4_0, the paged 4-bit
+        cache of KvCache (a seventh of the memory; the fp32 one is freed)."""
+        N.check(N.lib().brew_model_set_kv_cache(self.handle, int(qtype)), "set_kv_cache")
+
+    def score(self, tokens, top: int = 0):
+        """Log probabilities of tokens[1:] given the tokens before each, the
+        entropies of their distributions, and the `top` alternatives:
+        (logprob [n-1], entropy [n-1], ids [n-1][top], logprobs [n-1][top])."""
+        t = np.ascontiguousarray(tokens, np.int32)
+        k = max(t.size - 1, 0)
+        lp, ent = np.empty(k, np.float32), np.empty(k, np.float32)
+        ids, tops = np.empty((k, max(top, 0)), np.int32), np.empty((k, max(top, 0)), np.float32)
+        N.check(N.lib().brew_session_score(self.handle, _i32(t), t.size, top, _f32(lp), _f32(ent), _i32(ids), _f32(tops)),
+                "score")
+        return lp, ent, ids, tops
+
     def set_tp(self, comm: "Communicator") -> None:
         """Shards this model's matrices by rows over `comm` (every rank holds
         the same model); the forward then all-gathers each projection."""

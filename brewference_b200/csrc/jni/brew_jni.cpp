@@ -165,6 +165,36 @@ JNIEXPORT void JNICALL Java_com_epicmonstrosity_brewference_gpu_Brew_setPrefill(
     if (rc) throw_for(env, rc);
 }
 
+// brew_model_set_kv_cache: 0 (F32, the default) or 2 (Q4_0, the paged 4-bit cache).
+JNIEXPORT void JNICALL Java_com_epicmonstrosity_brewference_gpu_Brew_setKvCache(JNIEnv* env, jclass, jlong m,
+                                                                                jint type) {
+    const int rc = brew_model_set_kv_cache(reinterpret_cast<brew_model>(m), type);
+    if (rc) throw_for(env, rc);
+}
+
+// Log probabilities of tokens[1 ..] given the tokens before each, and the
+// entropies, into float[] of at least tokens.length - 1 (each may be null).
+// The arrays are not pinned: the call takes a forward for each token.
+JNIEXPORT void JNICALL Java_com_epicmonstrosity_brewference_gpu_Brew_score(JNIEnv* env, jclass, jlong m,
+                                                                           jintArray tokens, jfloatArray logprob,
+                                                                           jfloatArray entropy) {
+    const jsize n = tokens ? env->GetArrayLength(tokens) : 0;
+    if ((logprob && env->GetArrayLength(logprob) < n - 1) || (entropy && env->GetArrayLength(entropy) < n - 1)) {
+        jclass c = env->FindClass("java/lang/IllegalArgumentException");
+        if (c) env->ThrowNew(c, "an array shorter than the tokens to score");
+        return;
+    }
+    std::vector<int32_t> t(n > 0 ? n : 1);
+    if (n > 0) env->GetIntArrayRegion(tokens, 0, n, reinterpret_cast<jint*>(t.data()));
+    jfloat* lp = logprob ? env->GetFloatArrayElements(logprob, nullptr) : nullptr;
+    jfloat* en = entropy ? env->GetFloatArrayElements(entropy, nullptr) : nullptr;
+    const int rc = brew_session_score(reinterpret_cast<brew_model>(m), tokens ? t.data() : nullptr, n, 0, lp, en, nullptr,
+                                      nullptr);
+    if (lp) env->ReleaseFloatArrayElements(logprob, lp, rc ? JNI_ABORT : 0);
+    if (en) env->ReleaseFloatArrayElements(entropy, en, rc ? JNI_ABORT : 0);
+    if (rc) throw_for(env, rc);
+}
+
 // TransformerGraph.forward(token, pos) + Kernels.argMax; logits copied into
 // `logits` when it is not null.  Returns the argmax id.
 JNIEXPORT jint JNICALL Java_com_epicmonstrosity_brewference_gpu_Brew_forward(JNIEnv* env, jclass, jlong m, jint token,

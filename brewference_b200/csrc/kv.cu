@@ -352,6 +352,12 @@ KvView kv_view(const brew_kv_s* kv, int layer) {
     return v;
 }
 
+int kv_clear(brew_kv_s* kv, cudaStream_t s) {
+    BREW_CUDA(cudaMemsetAsync(kv->pool, 0, (size_t)kv->layer_bytes * kv->c.n_layers, s));
+    BREW_CUDA(cudaStreamSynchronize(s));
+    return BREW_OK;
+}
+
 bool kv_head_supported(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 256; }
 
 int kv_append_launch(int hd, const KvAppendParams& p, cudaStream_t s) {

@@ -86,6 +86,10 @@ struct KvAttendParams {
     uint32_t code_base;        // set by the launch
 };
 
+// The kernels' view of a cache's layer (kernels record bad rows in its own error word unless the caller sets another),
+// and every page zeroed in stream order.
+KvView kv_view(const brew_kv_s* kv, int layer);
+int kv_clear(brew_kv_s* kv, cudaStream_t s);
 int kv_append_launch(int head_size, const KvAppendParams& p, cudaStream_t s);
 int kv_attend_launch(int head_size, const KvAttendParams& p, cudaStream_t s);
 int64_t kv_attend_workspace(int head_size);

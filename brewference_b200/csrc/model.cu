@@ -20,9 +20,12 @@
 #include "eltwise.cuh"
 #include "gemm.cuh"
 #include "kqtc.cuh"
+#include "kv.cuh"
+#include "logprobs.cuh"
 #include "prefill.cuh"
 #include "tp.cuh"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -45,6 +48,14 @@ __global__ void step_kernel(int32_t* tokens, int32_t* pos, const int32_t* tok_sr
         tokens[0] = *tok_src;
         pos[0] = pos_val;
     }
+}
+
+// The rows of a prompt chunk of sequence 0: positions pos0 .. pos0 + n - 1.
+__global__ void chunk_rows_kernel(int32_t* rows, int pos0, int n) {
+    rows[0] = 0;
+    rows[1] = pos0;
+    rows[2] = 0;
+    rows[3] = n;
 }
 
 }  // namespace
@@ -148,6 +159,14 @@ struct brew_model_s {
     float *pf_x = nullptr, *pf_xn = nullptr, *pf_qkv = nullptr, *pf_xb = nullptr, *pf_xb2 = nullptr, *pf_h = nullptr;
     int8_t* pf_limbs = nullptr;
     float* pf_lsc = nullptr;
+    // paged 4-bit K/V cache in place of kc / vc (brew_model_set_kv_cache);
+    // the unfused forward then appends and attends through it
+    brew_kv kv = nullptr;
+    int32_t* kv_rows = nullptr;             // [max_batch] sequence ids, then of a prompt chunk [seq, pos, row0, end]
+    void* kv_ws = nullptr;                  // attention workspace
+    // token scores of one step (brew_session_score)
+    float* score_d = nullptr;               // [seq_len] log probabilities, [seq_len] entropies, then the top ones
+    int score_top = -1;
 };
 
 namespace brew {
@@ -499,6 +518,44 @@ int mv_w(brew_model_s* m, int which, int l, int64_t rows, int K, int64_t row0, i
     return mv_any(m, type, layer_ptr(t, l, rows, K) + row0 * row_bytes_of(type, K), x, ldx, K, n, y, ldy, B, s);
 }
 
+// Attention of layer l through the paged 4-bit cache: the rows' q (already
+// in [q | k | v] rows of stride qkvw) normalised and rotated in place, k and v
+// appended, then the attention into out.
+int kv_attention(brew_model_s* m, int l, float* qkv, float* out, const KvRowsDev& rows, cudaStream_t s) {
+    const brew_config& c = m->c;
+    const int hd = c.head_size, qw = c.n_heads * hd, kvd = c.n_kv_heads * hd;
+    const bool qknorm = arch_qknorm(c.arch);
+    KvAppendParams p = {};
+    p.kv = kv_view(m->kv, l);
+    p.kv.err = ctx().err_word;
+    p.rows = rows;
+    p.q = p.q_out = qkv;
+    p.k = qkv + qw;
+    p.v = qkv + qw + kvd;
+    p.ldq = p.ldkv = m->qkvw;
+    p.rope = !arch_rope_layer(c.arch, l) ? BREW_KV_ROPE_NONE
+             : arch_interleaved(c.arch)  ? BREW_KV_ROPE_INTERLEAVED
+                                         : BREW_KV_ROPE_HALF;
+    p.rope_scale = c.rope_scale > 0.0f ? c.rope_scale : 1.0f;
+    p.log2_base_hd =
+        std::log2((double)arch_rope_base(c.arch, c.rope_base, arch_gemma(c.arch) && !arch_global_layer(c.arch, l))) / hd;
+    p.qnorm = qknorm ? m->rms_q + (int64_t)l * hd : nullptr;
+    p.knorm = qknorm ? m->rms_k + (int64_t)l * hd : nullptr;
+    p.eps = c.eps;
+    KvAttendParams a = {};
+    a.kv = p.kv;
+    a.rows = rows;
+    a.q = qkv;
+    a.out = out;
+    a.ldq = m->qkvw;
+    a.ldo = qw;
+    a.window = arch_window(c.arch, l, c.sliding_window);
+    a.scale = 1.0f / (float)std::sqrt((double)hd);   // AttentionEngine.java:18-19
+    a.workspace = m->kv_ws;
+    int rc = kv_append_launch(hd, p, s);
+    return rc ? rc : kv_attend_launch(hd, a, s);
+}
+
 // The forward of a model with K-quant matrices (the Qwen2.5-7B Q4_K/Q6_K
 // config) and of tensor-parallel models: per layer, residual + RMSNorm (+ the
 // next tcgen05 K-quant matvec's x records) in one kernel, the q|k|v matvec
@@ -605,7 +662,9 @@ int enqueue_forward_unfused(brew_model_s* m, int B, bool with_classifier, cudaSt
             const TpSeg segs[3] = {{qs, 0, 0}, {ks, qs, qw}, {ks, qs + ks, qw + kvd}};
             if (!shard_attn && (rc = gather(sl, segs, 3, m->qkv, m->qkvw, 4 * l))) return rc;
         }
-        {
+        if (m->kv) {
+            if ((rc = kv_attention(m, l, q, m->xb, {m->kv_rows, m->pos_d, nullptr, B, B, 1}, s))) return rc;
+        } else {
             AttnParams a = {};
             a.batch = B;
             a.n_heads = c.n_heads;
@@ -1055,6 +1114,11 @@ int prefill_batched(brew_model_s* m, const int32_t* tok_d, int n, cudaStream_t s
         if ((rc = prefill_embed_launch(c.type_embed, m->t[T_EMBED]->d, c.vocab_size, dim, tok_d + c0, T, gemma, m->pf_x,
                                        err, s)))
             return rc;
+        if (m->kv) {
+            chunk_rows_kernel<<<1, 1, 0, s>>>(m->kv_rows + m->max_batch, c0, T);
+            BREW_CUDA(cudaGetLastError());
+            count_launch();
+        }
         for (int l = 0; l < L; ++l) {
             const bool global = arch_global_layer(c.arch, l);
             if ((rc = rmsnorm_launch(m->pf_x, dim, m->rms_att + (int64_t)l * dim, c.eps, dim, T, m->pf_xn, dim, s)) ||
@@ -1065,6 +1129,10 @@ int prefill_batched(brew_model_s* m, const int32_t* tok_d, int n, cudaStream_t s
                  (rc = add_bias_launch(m->pf_qkv + qw, qkvw, m->k_bias + (int64_t)l * kvd, kvd, T, s)) ||
                  (rc = add_bias_launch(m->pf_qkv + qw + kvd, qkvw, m->v_bias + (int64_t)l * kvd, kvd, T, s))))
                 return rc;
+            if (m->kv) {
+                const int32_t* r = m->kv_rows + m->max_batch;
+                if ((rc = kv_attention(m, l, m->pf_qkv, m->pf_xb, {r, r + 1, r + 2, 1, T, T}, s))) return rc;
+            } else {
             float* kcache = m->kc + (int64_t)l * c.seq_len * kvd;
             float* vcache = m->vc + (int64_t)l * c.seq_len * kvd;
             PfQkParams qk = {};
@@ -1102,6 +1170,7 @@ int prefill_batched(brew_model_s* m, const int32_t* tok_d, int n, cudaStream_t s
             at.xb = m->pf_xb;
             at.ldxb = qw;
             if ((rc = prefill_attn_launch(at, s))) return rc;
+            }
             if (l == L - 1) break;   // the rest of the last layer feeds only the logits
             if ((rc = gemm(1, l, m->pf_xb, qw, m->pf_xb2)) ||
                 (rc = residual_launch(m->pf_x, dim, m->pf_xb2, dim, gemma ? m->post_att + (int64_t)l * dim : nullptr,
@@ -1345,6 +1414,8 @@ void model_destroy(brew_model_s* m) {
             if (m->tp_peers.p[r] && m->tp_peers.p[r] != m->tp_arena) cudaIpcCloseMemHandle(m->tp_peers.p[r]);
     }
     for (void* p : m->allocs) cudaFree(p);
+    if (m->kv) brew_kv_free(m->kv);
+    if (m->score_d) cudaFree(m->score_d);
     if (m->h_pin) cudaFreeHost(m->h_pin);
     if (m->h_res) cudaFreeHost(m->h_res);
     if (m->prompt_d) cudaFree(m->prompt_d);
@@ -1498,6 +1569,7 @@ int brew_model_set_prefill(brew_model m, int32_t mode) {
 int brew_model_set_tp(brew_model m, brew_comm comm) {
     BREW_CHECK(m && comm, BREW_ERR_INVALID_ARG, "null argument");
     BREW_CHECK(!m->comm, BREW_ERR_INVALID_ARG, "the model is already sharded");
+    BREW_CHECK(!m->kv, BREW_ERR_UNSUPPORTED, "a model with a 4-bit K/V cache runs on one GPU");
     const brew_config& c = m->c;
     const int P = comm->nranks;
     const int qw = c.n_heads * c.head_size, kvd = c.n_kv_heads * c.head_size;
@@ -1625,6 +1697,111 @@ int brew_model_set_tp(brew_model m, brew_comm comm) {
     return BREW_OK;
 }
 
+int brew_model_set_kv_cache(brew_model m, int32_t type) {
+    BREW_CHECK(m, BREW_ERR_INVALID_ARG, "null model");
+    BREW_CHECK(type == BREW_TYPE_F32 || type == BREW_TYPE_Q4_0, BREW_ERR_UNSUPPORTED, "K/V cache of GGML type %d", type);
+    const brew_config& c = m->c;
+    BREW_CHECK(!m->comm, BREW_ERR_UNSUPPORTED, "the 4-bit K/V cache runs on one GPU (the model is sharded)");
+    if ((type == BREW_TYPE_Q4_0) == (m->kv != nullptr)) return BREW_OK;
+    BREW_CHECK(type == BREW_TYPE_Q4_0, BREW_ERR_UNSUPPORTED, "the model's fp32 K/V cache was given up");
+    BREW_CHECK(kv_head_supported(c.head_size), BREW_ERR_UNSUPPORTED, "K/V cache: head size %d (32, 64, 96, 128 or 256)",
+               c.head_size);
+    int rc = ensure_init();
+    if (rc) return rc;
+    std::lock_guard<std::mutex> lk(api_mutex());
+    BREW_CUDA(cudaDeviceSynchronize());
+    if ((rc = alloc_unfused(m))) return rc;
+    const int B = m->max_batch;
+    if (!m->kv_rows && (rc = dalloc(m, &m->kv_rows, (size_t)B + 4))) return rc;
+    std::vector<int32_t> ids(B);
+    for (int b = 0; b < B; ++b) ids[b] = b;
+    BREW_CUDA(cudaMemcpy(m->kv_rows, ids.data(), B * sizeof(int32_t), cudaMemcpyHostToDevice));
+    if (!m->kv_ws) {
+        uint8_t* ws = nullptr;
+        if ((rc = dalloc(m, &ws, (size_t)kv_attend_workspace(c.head_size)))) return rc;
+        m->kv_ws = ws;
+    }
+    const brew_kv_config kc = {c.n_layers, c.n_heads, c.n_kv_heads, c.head_size, B, c.seq_len, 64, 0};
+    brew_kv kv = nullptr;
+    if ((rc = brew_kv_create(&kc, &kv))) return rc;
+    for (int b = 0; b < B && !rc; ++b) rc = brew_kv_reserve(kv, b, c.seq_len, ctx().stream);
+    if (!rc && cudaStreamSynchronize(ctx().stream) != cudaSuccess) rc = set_error(BREW_ERR_CUDA, "K/V cache set-up");
+    if (rc) {
+        brew_kv_free(kv);
+        return rc;
+    }
+    // the forward changes: drop captured graphs and the decode kernel, and give the fp32 cache back
+    for (auto& g : m->graphs) cudaGraphExecDestroy(g.second);
+    m->graphs.clear();
+    m->graph_kernels.clear();
+    m->use_decode = false;
+    m->sess_pending = nullptr;
+    for (float** f : {&m->kc, &m->vc}) {
+        m->allocs.erase(std::find(m->allocs.begin(), m->allocs.end(), (void*)*f));
+        cudaFree(*f);
+        *f = nullptr;
+    }
+    m->dp.kc = m->dp.vc = nullptr;
+    m->kv = kv;
+    return BREW_OK;
+}
+
+int brew_session_score(brew_model m, const int32_t* tokens, int32_t n, int32_t top, float* logprob, float* entropy,
+                       int32_t* top_ids, float* top_logprobs) {
+    BREW_CHECK(m && tokens, BREW_ERR_INVALID_ARG, "null argument");
+    BREW_CHECK(n >= 2, BREW_ERR_INVALID_ARG, "%d tokens: the first one has no log probability", n);
+    BREW_CHECK(n - 1 <= m->c.seq_len, BREW_ERR_CONTEXT_FULL, "The session has reached its context limit of %d tokens.",
+               m->c.seq_len);
+    BREW_CHECK(top >= 0 && top <= BREW_MAX_TOP && top <= m->c.vocab_size, BREW_ERR_INVALID_ARG, "%d alternatives (at most %d)",
+               top, std::min(BREW_MAX_TOP, m->c.vocab_size));
+    BREW_CHECK(logprob || entropy || top > 0, BREW_ERR_INVALID_ARG, "nothing is asked");
+    BREW_CHECK(top == 0 || (top_ids && top_logprobs), BREW_ERR_INVALID_ARG, "top_ids and top_logprobs must be given");
+    for (int i = 0; i < n; ++i)
+        BREW_CHECK(tokens[i] >= 0 && tokens[i] < m->c.vocab_size, BREW_ERR_INVALID_ARG, "token %d out of range", tokens[i]);
+    int rc = ensure_init();
+    if (rc) return rc;
+    std::lock_guard<std::mutex> lk(api_mutex());
+    cudaStream_t s = ctx().stream;
+    const size_t cap = m->c.seq_len;
+    if (m->score_top < top) {   // [log probabilities | entropies | alternatives | their log probabilities]
+        if (m->score_d) cudaFree(m->score_d);
+        m->score_d = nullptr;
+        m->score_top = -1;
+        BREW_CUDA(cudaMalloc(&m->score_d, cap * (2 + 2 * (size_t)top) * sizeof(float)));
+        m->score_top = top;
+    }
+    float* lp = m->score_d;
+    float* en = lp + cap;
+    int32_t* ids = reinterpret_cast<int32_t*>(en + cap);
+    float* tl = en + cap + cap * top;
+    m->sess_pending = nullptr;   // the cache holds another text
+    if (m->prompt_cap < n + 1) {
+        if (m->prompt_d) cudaFree(m->prompt_d);
+        m->prompt_d = nullptr;
+        m->prompt_cap = 0;
+        BREW_CUDA(cudaMalloc(&m->prompt_d, (size_t)(n + 1) * sizeof(int32_t)));
+        m->prompt_cap = n + 1;
+    }
+    BREW_CUDA(cudaMemcpyAsync(m->prompt_d, tokens, (size_t)n * sizeof(int32_t), cudaMemcpyHostToDevice, s));
+    const int V = m->c.vocab_size;
+    for (int i = 0; i + 1 < n; ++i) {
+        const LogprobsParams p = {m->logits, V, V, 1, m->prompt_d + i + 1, lp + i, en + i, top, ids + (int64_t)i * top,
+                                  tl + (int64_t)i * top};
+        if ((rc = launch_step(m, m->prompt_d + i, i, nullptr, s)) || (rc = launch_forward(m, 1, true, s)) ||
+            (rc = logprobs_launch(p, s)))
+            return rc;
+    }
+    const size_t k = n - 1;
+    if (logprob) BREW_CUDA(cudaMemcpyAsync(logprob, lp, k * sizeof(float), cudaMemcpyDeviceToHost, s));
+    if (entropy) BREW_CUDA(cudaMemcpyAsync(entropy, en, k * sizeof(float), cudaMemcpyDeviceToHost, s));
+    if (top > 0) {
+        BREW_CUDA(cudaMemcpyAsync(top_ids, ids, k * top * sizeof(int32_t), cudaMemcpyDeviceToHost, s));
+        BREW_CUDA(cudaMemcpyAsync(top_logprobs, tl, k * top * sizeof(float), cudaMemcpyDeviceToHost, s));
+    }
+    BREW_CUDA(cudaStreamSynchronize(s));
+    return after_step_check(m, "brew_session_score");
+}
+
 int brew_model_tensor(brew_model m, int which, brew_tensor* out) {
     BREW_CHECK(m && out && which >= 0 && which < T_COUNT, BREW_ERR_INVALID_ARG, "bad argument");
     *out = m->t[which];
@@ -1652,6 +1829,7 @@ int brew_model_set_trace(brew_model m, int32_t on) {
 int brew_model_reset(brew_model m) {
     BREW_CHECK(m, BREW_ERR_INVALID_ARG, "null model");
     std::lock_guard<std::mutex> lk(api_mutex());
+    if (m->kv) return kv_clear(m->kv, ctx().stream);
     BREW_CUDA(cudaMemsetAsync(m->kc, 0, (size_t)m->max_batch * m->cache_bstride * sizeof(float), ctx().stream));
     BREW_CUDA(cudaMemsetAsync(m->vc, 0, (size_t)m->max_batch * m->cache_bstride * sizeof(float), ctx().stream));
     BREW_CUDA(cudaStreamSynchronize(ctx().stream));

@@ -367,6 +367,24 @@ BREW_API int brew_session_decode(brew_model m, int32_t n_steps, int32_t* out_tok
 #define BREW_PREFILL_TOKENS 0
 #define BREW_PREFILL_BATCHED 1
 BREW_API int brew_model_set_prefill(brew_model m, int32_t mode);
+/* The model's K/V cache.  BREW_TYPE_F32 (the default): dense fp32, as the
+ * reference's RunState.  BREW_TYPE_Q4_0: the paged 4-bit cache of brew_kv_*
+ * (0.14 of the bytes; the fp32 cache is freed and the session forgotten, and
+ * the model stays with it); every forward, prefill (both modes) and session
+ * call then goes through brew_kv_append_dev's and brew_kv_attend_dev's
+ * kernels in the kernel-graph forward.  K and V are rounded to 4 bits, so
+ * logits differ from the fp32 cache's (brew_session_score shows by how much
+ * on a text).  One GPU; head sizes 32, 64, 96, 128, 256; else
+ * BREW_ERR_UNSUPPORTED.  No reference counterpart. */
+BREW_API int brew_model_set_kv_cache(brew_model m, int32_t type);
+/* Scores a text: tokens[i] is forwarded at position i for i < n - 1, and
+ * logprob[i] = log p(tokens[i + 1] | tokens[0 .. i]), with the entropy and the
+ * `top` alternatives of the same distribution (brew_logprobs_dev); host
+ * arrays of n - 1 entries (top_ids / top_logprobs [n - 1][top]), each of the
+ * three optional.  Uses sequence 0 and ends its session.  n - 1 <= seq_len,
+ * else BREW_ERR_CONTEXT_FULL. */
+BREW_API int brew_session_score(brew_model m, const int32_t* tokens, int32_t n, int32_t top, float* logprob,
+                                float* entropy, int32_t* top_ids, float* top_logprobs);
 /* Kernels in one decode step's CUDA graph (for launch accounting). */
 BREW_API int brew_model_step_kernels(brew_model m, int32_t batch, int32_t* n_kernels);
 
