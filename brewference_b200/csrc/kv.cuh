@@ -84,6 +84,8 @@ struct KvAttendParams {
     float scale;
     void* workspace;
     uint32_t code_base;        // set by the launch
+    int64_t pairs_min;         // entries of fewer (row, head) pairs a kv head are the single-token kernel's, the others
+                               // the prompt kernel's
 };
 
 // The kernels' view of a cache's layer (kernels record bad rows in its own error word unless the caller sets another),
@@ -94,6 +96,11 @@ int kv_append_launch(int head_size, const KvAppendParams& p, cudaStream_t s);
 int kv_attend_launch(int head_size, const KvAttendParams& p, cudaStream_t s);
 int64_t kv_attend_workspace(int head_size);
 bool kv_head_supported(int head_size);
+// The prompt kernel (tcgen05), its part of the workspace: kv_attend_launch's.
+constexpr int KV_COUNTER_BYTES = 4096;
+bool kv_prefill_supported(int head_size);
+int64_t kv_prefill_workspace(int head_size);
+int kv_prefill_launch(int head_size, const KvAttendParams& p, cudaStream_t s);
 
 // Entry i of a call, checked: its rows lie in the buffers, its sequence in
 // the cache and its positions in reserved pages.  A bad entry has no rows.
