@@ -67,6 +67,15 @@ struct PfRest {
     uint32_t poison[4][PF_GROUPS];   // its V rows with a NaN scale, a bit each
 };
 
+// True in one lane.  In a branch on it the compiler keeps an MMA's operands in
+// uniform registers: 37 cycles from one M128 N64 K16 to the next, 56 in a
+// branch on the lane's number.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p = 0;
+    asm volatile(
+        "{\n\t.reg .b32 r;\n\t.reg .pred q;\n\telect.sync r|q, 0xffffffff;\n\t@q mov.u32 %0, 1;\n\t}" : "+r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -97,14 +106,28 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8])
                  : "memory");
 }
 
+// One try of at most about 0.1 ms in which the thread sleeps: polling warps
+// would take issue slots and shared-memory cycles from the working ones.
+__device__ __forceinline__ bool pf_try(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(100000u)
+        : "memory");
+    return ok != 0;
+}
+
 // Waits for a phase, at most a second, or until another warp of the CTA has
 // given up (which is recorded).
 __device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t parity, PfRest& s, unsigned int* err) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (pf_try(bar, parity)) return true;
     const uint64_t t0 = global_ns();
     for (uint32_t it = 0; it < BREW_SPIN_LIMIT; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 63u) == 63u && (ld_volatile_int(&s.abort) || global_ns() - t0 > 1000000000ull)) break;
+        if (pf_try(bar, parity)) return true;
+        if (ld_volatile_int(&s.abort) || global_ns() - t0 > 1000000000ull) break;
     }
     s.abort = 1;
     atomicOr(err, BREW_DEVERR_TIMEOUT_FULL);
@@ -221,46 +244,53 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
         }
     } else if (warp == 1) {
         // ---------------- MMA issue ----------------
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
             constexpr uint32_t iqk = umma_idesc_f16(PF_M, PF_KT), ipv = umma_idesc_f16(PF_M, HD);
-            const uint32_t kb = smem_u32(smem + S::K), vb = smem_u32(smem + S::V);
+            const uint64_t kdesc = umma_desc_k(smem_u32(smem + S::K), S::K_PIECE, 128);
+            const uint64_t vdesc = umma_desc_k(smem_u32(smem + S::V), S::V_PIECE, S::V_GROUP);
             auto qk = [&](int i) -> bool {
                 const int b = i & 1;
-                if (!pf_wait(&sh.k_full[b], i >> 1 & 1, sh, kv.err) || !pf_wait(&sh.s_empty[b], (i >> 1 & 1) ^ 1, sh, kv.err))
+                if (!pf_wait_warp(&sh.k_full[b], i >> 1 & 1, sh, kv.err) ||
+                    !pf_wait_warp(&sh.s_empty[b], (i >> 1 & 1) ^ 1, sh, kv.err))
                     return false;
                 tc_fence_after();
-                const uint32_t hi = kb + b * 2 * S::K_PART, lo = hi + S::K_PART, d = tmem + PF_T_S + b * PF_KT;
+                if (elect_one()) {
+                    const uint64_t hi = kdesc + b * (2 * S::K_PART / 16);
+                    const uint32_t d = tmem + PF_T_S + b * PF_KT;
 #pragma unroll
-                for (int pass = 0; pass < 3; ++pass)
+                    for (int pass = 0; pass < 3; ++pass)
 #pragma unroll
-                    for (int s = 0; s < HD / 16; ++s)
-                        umma_f16_ts(d, tmem + (pass == 0 ? PF_T_QL : PF_T_QH) + 8 * s,
-                                    umma_desc_k((pass == 1 ? lo : hi) + s * 2 * S::K_PIECE, S::K_PIECE, 128), iqk,
-                                    pass + s > 0);
-                umma_commit(&sh.s_full[b]);
-                umma_commit(&sh.k_empty[b]);
+                        for (int s = 0; s < HD / 16; ++s)
+                            umma_f16_ts(d, tmem + (pass == 0 ? PF_T_QL : PF_T_QH) + 8 * s,
+                                        hi + ((pass == 1 ? S::K_PART : 0) + s * 2 * S::K_PIECE) / 16, iqk, pass + s > 0);
+                    umma_commit(&sh.s_full[b]);
+                    umma_commit(&sh.k_empty[b]);
+                }
+                __syncwarp();
                 return true;
             };
             auto pv = [&](int i) -> bool {
                 const int b = i & 1;
-                if (!pf_wait(&sh.p_full, i & 1, sh, kv.err) || !pf_wait(&sh.v_full[b], i >> 1 & 1, sh, kv.err) ||
-                    !pf_wait(&sh.o_empty, (i & 1) ^ 1, sh, kv.err))
+                if (!pf_wait_warp(&sh.p_full, i & 1, sh, kv.err) || !pf_wait_warp(&sh.v_full[b], i >> 1 & 1, sh, kv.err) ||
+                    !pf_wait_warp(&sh.o_empty, (i & 1) ^ 1, sh, kv.err))
                     return false;
                 tc_fence_after();
-                const uint32_t hi = vb + b * 2 * S::V_PART, lo = hi + S::V_PART;
+                if (elect_one()) {
+                    const uint64_t hi = vdesc + b * (2 * S::V_PART / 16);
 #pragma unroll
-                for (int pass = 0; pass < 3; ++pass)
+                    for (int pass = 0; pass < 3; ++pass)
 #pragma unroll
-                    for (int s = 0; s < PF_KT / 16; ++s)
-                        umma_f16_ts(tmem + PF_T_O, tmem + (pass == 0 ? PF_T_PL : PF_T_PH) + 8 * s,
-                                    umma_desc_k((pass == 1 ? lo : hi) + s * 2 * S::V_PIECE, S::V_PIECE, S::V_GROUP), ipv,
-                                    pass + s > 0);
-                umma_commit(&sh.o_full);
-                umma_commit(&sh.v_empty[b]);
-                umma_commit(&sh.p_empty);
+                        for (int s = 0; s < PF_KT / 16; ++s)
+                            umma_f16_ts(tmem + PF_T_O, tmem + (pass == 0 ? PF_T_PL : PF_T_PH) + 8 * s,
+                                        hi + ((pass == 1 ? S::V_PART : 0) + s * 2 * S::V_PIECE) / 16, ipv, pass + s > 0);
+                    umma_commit(&sh.o_full);
+                    umma_commit(&sh.v_empty[b]);
+                    umma_commit(&sh.p_empty);
+                }
+                __syncwarp();
                 return true;
             };
-            bool ok = pf_wait(&sh.q_full, 0, sh, kv.err) && qk(0);
+            bool ok = pf_wait_warp(&sh.q_full, 0, sh, kv.err) && qk(0);
             for (int i = 0; i < n && ok; ++i) ok = (i + 1 >= n || qk(i + 1)) && pv(i);
         }
         __syncwarp();
