@@ -14,14 +14,20 @@
 // starts at 0 and is added in fp32 registers with the softmax's correction,
 // because accumulation in tensor memory truncates.
 //
-// Warps: one copies the tiles' packed groups (bulk copies), one thread issues
-// the MMAs, four make the softmax (a thread is a row), eight add up O (a
-// thread is half a row), four unpack K and V.  K, V, S and the packed tiles
-// are buffered twice or more; QK of the next tile is issued before PV of the
+// The tiles of all items, end to end, are cut into one equal run a CTA; items
+// that a cut divides leave parts (O, maximum, sum) in the workspace, which the
+// last of their CTAs joins.
+//
+// Warps: one copies the tiles' packed groups (bulk copies), one issues the
+// MMAs, two warpgroups take turns at the softmax of a tile (a thread is a row;
+// the running maximum passes between them), two add up O (a thread is half a
+// row), two take turns at unpacking a tile's K and V and at bringing an item's
+// q.  K, V, S, P and the packed tiles are buffered twice or more and the rings
+// go on from item to item; QK of the next tile is issued before PV of the
 // present one, so the tensor cores work while the softmax does.
 //
-// Bound: the tensor cores, 1536 cycles a tile of 64 keys x 128 pairs x 128
-// dims (3 + 3 products), beside about 3400 instructions of the 16 warps.
+// Bound: the tensor cores, 1730 cycles a tile of 64 keys x 128 pairs x 128
+// dims (24 products of 64 columns at 37, 12 of 128 at 70).
 #include <algorithm>
 
 #include "brew_internal.cuh"
@@ -35,15 +41,23 @@ namespace {
 constexpr int PF_M = 128;              // pairs of an item
 constexpr int PF_KT = 64;              // keys of a tile
 constexpr int PF_GROUPS = PF_KT / KV_GROUP;
-constexpr int PF_RAW = 3;              // packed tiles in flight
-constexpr int PF_WARPS = 18;
-constexpr int PF_THREADS = 32 * PF_WARPS;
-constexpr int PF_W_SUM = 6, PF_W_UNPACK = 14;   // first warps of the sums and the unpacking (0 copies, 1 issues)
+constexpr int PF_RAW = 4;              // packed tiles in flight
+constexpr int PF_MAX_CTAS = 148;
+constexpr int PF_RUN = 4;              // tiles of a run, at least
+constexpr int PF_ITEM = 4;             // what an item costs beside its tiles, in tiles
 constexpr float PF_PLOG2 = 9.0f;       // p is carried times 2^9 (2^13 in tiles whose values are taken 2^-4)
-constexpr int PF_MAX_PARTS = 148;      // parts of split items
+constexpr int PF_QS = 36, PF_OS = 20;  // floats from row to row where q and the output are turned: no bank twice
 
-// Tensor memory: S twice, O, q's parts, p's parts.
-constexpr uint32_t PF_T_S = 0, PF_T_O = 128, PF_T_QH = 256, PF_T_QL = 320, PF_T_PH = 384, PF_T_PL = 416;
+// Seven warpgroups; the first warp of each kind, and the registers of its
+// threads (the sum over the warpgroups is what the block is launched with).
+constexpr int PF_W_SOFT = 4, PF_W_SUM = 12, PF_W_UNPACK = 20, PF_THREADS = 896;
+constexpr int PF_ITEM_USERS = 3 + 24;   // warps that walk the run's items
+constexpr int PF_REGS = 72, PF_REGS_ISSUE = 40, PF_REGS_SOFT = 80, PF_REGS_SUM = 88, PF_REGS_UNPACK = 64;
+static_assert(PF_RAW <= 4, "rings of 4");
+static_assert(PF_REGS_ISSUE + 2 * (PF_REGS_SOFT + PF_REGS_SUM + PF_REGS_UNPACK) <= 7 * PF_REGS, "registers");
+
+// Tensor memory: S twice, O, q's parts, p's parts twice.
+constexpr uint32_t PF_T_S = 0, PF_T_O = 128, PF_T_QH = 256, PF_T_QL = 320, PF_T_P = 384;
 
 template <int R>
 struct PfShape {
@@ -53,18 +67,38 @@ struct PfShape {
     // groups of 8 dims 16 bytes further apart: the unpacking warps' stores fall into different banks
     static constexpr int K_PIECE = PF_KT * 16 + 32, K_PART = HD / 8 * K_PIECE;
     static constexpr int V_GROUP = 144, V_PIECE = HD / 8 * V_GROUP, V_PART = PF_KT / 8 * V_PIECE;
-    static constexpr int K = PF_RAW * RAW_BYTES, V = K + 4 * K_PART, REST = V + 4 * V_PART;
+    static constexpr int K = PF_RAW * RAW_BYTES, V = K + 4 * K_PART, QSTAGE = V + 4 * V_PART;
+    static constexpr int OSTAGE = QSTAGE + 4 * 32 * PF_QS * 4, REST = OSTAGE + 8 * 32 * PF_OS * 4;
+};
+
+// The (row, head) pairs of one (entry, kv head), 128 at a time, and the part
+// of their keys that this CTA's run of tiles covers.
+struct PfItem {
+    KvEntry e;
+    int b, hk, mt;       // entry, kv head, which 128 pairs
+    int off;             // the item's first tile, counted from the run's beginning (negative: others have its beginning)
+    int cnt;             // its tiles
+    int pr0, npairs;
+    int kmin, kmax;      // the keys that some pair sees
+    int all_lo, all_hi;  // the keys that every pair sees
+    int ta, n;           // the run's tiles of it
 };
 
 struct PfRest {
     uint64_t raw_full[PF_RAW], raw_empty[PF_RAW], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_empty[2];
-    uint64_t q_full, p_full, p_empty, o_full, o_empty, fin;
+    uint64_t p_full[2], p_empty[2], meta_full[4], ml_full[2], ml_empty[2], m_full[2][4], item_full[4], item_empty[4], part_full, last_full, q_full, q_empty[4], o_full[2], o_empty[2];
+    uint64_t poison[4];         // of tile i & 3: its V rows with a NaN scale, a bit each
+    int64_t all;                // the call's tiles and items' costs
+    int ctas, len;              // CTAs that have some; this one's part
+    PfItem item[4];             // of item j & 3
     uint32_t tmem;
     int last;
-    int abort;
-    float corr[2][PF_M], m[PF_M], l[PF_M];
     float unscale[4];           // of tile i & 3: 16 where its values are taken times 2^-4
-    uint32_t poison[4][PF_GROUPS];   // its V rows with a NaN scale, a bit each
+    float corr[4][PF_M];        // of tile i & 3: what O so far is multiplied by
+    float m[2][PF_M];           // the running maximum behind tile i & 1
+    float qmax[PF_M];           // the largest magnitudes of the item's q rows
+    float sfac[4][PF_M];        // of item j & 3: scores are the products times this (log2)
+    float2 ml[2][2][PF_M];      // of item j & 1 and a softmax warpgroup: maximum and sum of its tiles
 };
 
 // True in one lane.  In a branch on it the compiler keeps an MMA's operands in
@@ -106,39 +140,188 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8])
                  : "memory");
 }
 
-// One try of at most about 0.1 ms in which the thread sleeps: polling warps
-// would take issue slots and shared-memory cycles from the working ones.
-__device__ __forceinline__ bool pf_try(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(100000u)
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
         : "memory");
-    return ok != 0;
+}
+__device__ __forceinline__ float2 f2_float2(uint64_t x) {
+    float2 d;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(x));
+    return d;
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// Waits for a phase, at most a second, or until another warp of the CTA has
-// given up (which is recorded).
-__device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t parity, PfRest& s, unsigned int* err) {
-    if (pf_try(bar, parity)) return true;
-    const uint64_t t0 = global_ns();
-    for (uint32_t it = 0; it < BREW_SPIN_LIMIT; ++it) {
-        if (pf_try(bar, parity)) return true;
-        if (ld_volatile_int(&s.abort) || global_ns() - t0 > 1000000000ull) break;
+// Waits for a phase, some 4 million tries of at most a microsecond in which the
+// warp sleeps (polling warps would take issue slots and shared-memory cycles
+// from the working ones); false, in all lanes and recorded, if it does not
+// come: the warp then leaves, and so, one after the other, do those that wait
+// for it.  (Few instructions: the kernel's loops have to stay in the
+// instruction cache together, and what follows a wait waits for its fetch.)
+constexpr uint32_t PF_TRIES = 1u << 22;
+__device__ __forceinline__ bool pf_wait_warp(uint64_t* bar, uint32_t parity, unsigned int* err) {
+#pragma unroll 1
+    for (uint32_t it = 0; it < PF_TRIES; ++it) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(1000u)
+            : "memory");
+        if (__all_sync(0xffffffffu, ok)) return true;
     }
-    s.abort = 1;
     atomicOr(err, BREW_DEVERR_TIMEOUT_FULL);
     return false;
 }
-__device__ __forceinline__ bool pf_wait_warp(uint64_t* bar, uint32_t parity, PfRest& s, unsigned int* err) {
-    return __all_sync(0xffffffffu, pf_wait(bar, parity, s, err));
+
+__device__ __forceinline__ void pf_range(const KvAttendParams& p, const KvEntry& e, int G, int mt, int& all_hi, int& kmin,
+                                         int& kmax) {
+    const int pr0 = mt * PF_M;
+    all_hi = e.pos0 + pr0 / G;
+    kmax = e.pos0 + (min(e.rows * G, pr0 + PF_M) - 1) / G;
+    kmin = p.window > 0 ? max(0, all_hi - p.window + 1) : 0;
+}
+__device__ __forceinline__ void pf_set(const KvAttendParams& p, int G, int len, PfItem& x) {
+    pf_range(p, x.e, G, x.mt, x.all_hi, x.kmin, x.kmax);
+    x.pr0 = x.mt * PF_M;
+    x.npairs = min(x.e.rows * G - x.pr0, PF_M);
+    x.all_lo = p.window > 0 ? max(0, x.kmax - p.window + 1) : 0;
+    x.cnt = x.kmax / PF_KT + 1 - x.kmin / PF_KT;
+    const int first = max(0, -x.off);
+    x.ta = x.kmin / PF_KT + first;
+    x.n = min(x.cnt, len - x.off) - first;
+}
+// False behind the run's last item.
+__device__ __forceinline__ bool pf_next(const KvAttendParams& p, int G, int len, PfItem& x) {
+    x.off += x.cnt + PF_ITEM;
+    if (x.off >= len) return false;
+    if (++x.mt >= (x.e.rows * G + PF_M - 1) / PF_M) {
+        x.mt = 0;
+        if (++x.hk >= p.kv.n_kv) {
+            x.hk = 0;
+            do {
+                if (++x.b >= p.rows.n_seqs) return false;
+                x.e = kv_check_entry(p.kv, p.rows, x.b);
+            } while ((int64_t)x.e.rows * G < p.pairs_min);
+        }
+    }
+    pf_set(p, G, len, x);
+    return true;
+}
+
+// Item j of the run (n = 0: behind the last), and giving its slot back.
+__device__ __forceinline__ bool pf_item(PfRest& sh, int j, PfItem& x, unsigned int* err) {
+    if (!pf_wait_warp(&sh.item_full[j & 3], j >> 2 & 1, err)) return false;
+    x = sh.item[j & 3];
+    return x.n > 0;
+}
+__device__ __forceinline__ void pf_item_done(PfRest& sh, int j, int lane) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.item_empty[j & 3]);
+}
+
+// The item's q rows to tensor memory: two fp16 parts times a power of two,
+// amax * f in [2^13, 2^14).  A warp brings 32 rows, 32 dims of 4 rows a load,
+// and turns them (lane = row) in shared memory: with a row a lane, a warp's
+// loads would touch 32 lines each (4.6 us an item).
+template <int R>
+__device__ __forceinline__ void pf_q_at(const KvAttendParams& p, const PfItem& x, int G, int r, int64_t& at) {
+    const int pi = x.pr0 + min(r, x.npairs - 1), qr = pi / G;   // missing pairs repeat the last one
+    at = (int64_t)(x.e.row0 + qr) * p.ldq + (int64_t)(x.hk * G + pi - qr * G) * (32 * R);
+}
+__device__ __forceinline__ void pf_q_load(const KvAttendParams& p, int64_t row_at, int d, int lane, float4 (&v)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)   // dims d .. d + 31 of rows 4 k + lane / 8
+        v[k] = *reinterpret_cast<const float4*>(p.q + __shfl_sync(0xffffffffu, row_at, 4 * k + (lane >> 3)) + d + 4 * (lane & 7));
+}
+// The rows' largest magnitudes, before the last item's products are made.
+template <int R>
+__device__ __forceinline__ void pf_q_max(const KvAttendParams& p, PfRest& sh, const PfItem& x, int G, int w, int lane) {
+    int64_t row_at;
+    pf_q_at<R>(p, x, G, 32 * w + lane, row_at);
+    float amax[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) amax[k] = 0.0f;
+#pragma unroll 1
+    for (int d = 0; d < 32 * R; d += 32) {
+        float4 v[8];
+        pf_q_load(p, row_at, d, lane, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            amax[k] = fmaxf(amax[k], fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w))));
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) amax[k] = fmaxf(amax[k], __shfl_xor_sync(0xffffffffu, amax[k], o));
+        if ((lane & 7) == k) sh.qmax[32 * w + 4 * k + (lane >> 3)] = amax[k];
+    }
+    __syncwarp();
+}
+template <int R>
+__device__ __forceinline__ bool pf_q_store(const KvAttendParams& p, PfRest& sh, float* stage, uint32_t tmem, const PfItem& x, int G,
+                                           int j, int w, int lane) {
+    const int r = 32 * w + lane;
+    int64_t row_at;
+    pf_q_at<R>(p, x, G, r, row_at);
+    stage += w * 32 * PF_QS;
+    float4 v[8];
+    pf_q_load(p, row_at, 0, lane, v);
+    const int fe = min(253, max(1, 267 - (int)(__float_as_uint(sh.qmax[r]) >> 23)));
+    const float f = copysignf(__uint_as_float((uint32_t)fe << 23), p.scale);
+    // the last item's products are made, and sfac of four items before is read: the products of its tiles' successors
+    // waited for that
+    if (j > 0 && !pf_wait_warp(&sh.q_empty[(j - 1) & 3], (j - 1) >> 2 & 1, p.kv.err)) return false;
+    tc_fence_after();
+    // (never 0: a masked score is -inf times it)
+    sh.sfac[j & 3][r] = fmaxf(fabsf(p.scale) * 1.44269504088896341f * __uint_as_float((uint32_t)(254 - fe) << 23), 1e-36f);
+    const uint32_t tq = tmem + ((uint32_t)(32 * w) << 16);
+#pragma unroll 1
+    for (int d = 0; d < 32 * R; d += 32) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            *reinterpret_cast<float4*>(stage + (4 * k + (lane >> 3)) * PF_QS + 4 * (lane & 7)) = v[k];
+        __syncwarp();
+        if (d + 32 < 32 * R) pf_q_load(p, row_at, d + 32, lane, v);
+#pragma unroll 1
+        for (int c = 0; c < 32; c += 16) {   // dims (0, 4 | 1, 5 | 2, 6 | 3, 7) of each 8, as K's are unpacked
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 y = *reinterpret_cast<const float4*>(stage + lane * PF_QS + c + 8 * h);
+                const float4 z = *reinterpret_cast<const float4*>(stage + lane * PF_QS + c + 8 * h + 4);
+                split_half2(y.x * f, z.x * f, hi[4 * h], lo[4 * h]);
+                split_half2(y.y * f, z.y * f, hi[4 * h + 1], lo[4 * h + 1]);
+                split_half2(y.z * f, z.z * f, hi[4 * h + 2], lo[4 * h + 2]);
+                split_half2(y.w * f, z.w * f, hi[4 * h + 3], lo[4 * h + 3]);
+            }
+            tmem_st8(tq + PF_T_QH + (d + c) / 2, hi);
+            tmem_st8(tq + PF_T_QL + (d + c) / 2, lo);
+        }
+        __syncwarp();
+    }
+    tmem_st_wait();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.q_full);
+    return true;
 }
 
 template <int R>
-__global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_constant__ KvAttendParams p, int splits) {
+__global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_constant__ KvAttendParams p) {
     using S = PfShape<R>;
     constexpr int HD = S::HD;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -147,50 +330,100 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n_kv = kv.n_kv, G = kv.n_heads / n_kv;
 
-    // ---- this CTA's item: the entries' items end to end, the long ones of each first
-    const int split = blockIdx.x % splits;
-    int64_t rel = blockIdx.x / splits;
-    const int64_t item = rel;
-    KvEntry e = {};
-    int tiles_m = 0;
-    for (int b0 = 0; b0 < p.rows.n_seqs; b0 += 32) {   // every warp for itself, 32 entries at a time
-        int mine = 0;
-        if (b0 + lane < p.rows.n_seqs) {
-            const KvEntry x = kv_check_entry(kv, p.rows, b0 + lane);   // (the other kernel of the call records bad ones)
-            if ((int64_t)x.rows * G >= p.pairs_min) mine = (int)(((int64_t)x.rows * G + PF_M - 1) / PF_M);
-        }
-        int inc = mine;
+    if (warp == 0) {
+        // ---- the run: the tiles of all items end to end (entries, kv heads, pairs, keys), before each item's what it
+        // costs besides, cut into equal parts
+        auto entry_tiles = [&](int b) -> int64_t {   // of one kv head; 0: the other kernel's (which records bad entries)
+            int64_t t = 0;
+            if (b < p.rows.n_seqs) {
+                const KvEntry e = kv_check_entry(kv, p.rows, b);
+                if ((int64_t)e.rows * G >= p.pairs_min)
+#pragma unroll 1
+                    for (int mt = 0; mt * PF_M < e.rows * G; ++mt) {
+                        int hi, kmin, kmax;
+                        pf_range(p, e, G, mt, hi, kmin, kmax);
+                        t += PF_ITEM + kmax / PF_KT + 1 - kmin / PF_KT;
+                    }
+            }
+            return t;
+        };
+        auto scan = [&](int64_t x) {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int t = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += t;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t t = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += t;
+            }
+            return x;
+        };
+        int64_t all = 0, mine = 0, inc = 0;
+        int items = 0;
+#pragma unroll 1
+        for (int b0 = 0; b0 < p.rows.n_seqs; b0 += 32) {
+            mine = entry_tiles(b0 + lane);
+            inc = scan(mine);
+            all += __shfl_sync(0xffffffffu, inc, 31) * n_kv;
+            items += __popc(__ballot_sync(0xffffffffu, mine > 0));
         }
-        const int64_t all = (int64_t)__shfl_sync(0xffffffffu, inc, 31) * n_kv;
-        if (rel >= all) {
-            rel -= all;
-            continue;
+        // fewer CTAs for little work: a cut item costs its join
+        const int ctas = (int)min((int64_t)gridDim.x, max((int64_t)items * n_kv, (all + PF_RUN - 1) / PF_RUN));
+        const int64_t t0 = all * blockIdx.x / max(ctas, 1), t1 = all * (blockIdx.x + 1) / max(ctas, 1);
+        int len = blockIdx.x < ctas ? (int)(t1 - t0) : 0;
+        if (len > 0) {
+            int64_t rel = t0;
+#pragma unroll 1
+            for (int b0 = 0; b0 < p.rows.n_seqs; b0 += 32) {
+                if (p.rows.n_seqs > 32) {
+                    mine = entry_tiles(b0 + lane);
+                    inc = scan(mine);
+                }
+                const int64_t here = __shfl_sync(0xffffffffu, inc, 31) * n_kv;
+                if (rel >= here) {
+                    rel -= here;
+                    continue;
+                }
+                const int at = __ffs(__ballot_sync(0xffffffffu, inc * n_kv > rel)) - 1;
+                rel -= __shfl_sync(0xffffffffu, inc - mine, at) * n_kv;
+                const int64_t head = __shfl_sync(0xffffffffu, mine, at);
+                const KvEntry e = kv_check_entry(kv, p.rows, b0 + at);
+                const int hk = (int)(rel / head);
+                rel -= hk * head;
+#pragma unroll 1
+                for (int m0 = 0;; m0 += 32) {
+                    int cnt = 0;
+                    if ((m0 + lane) * PF_M < e.rows * G) {
+                        int hi, kmin, kmax;
+                        pf_range(p, e, G, m0 + lane, hi, kmin, kmax);
+                        cnt = PF_ITEM + kmax / PF_KT + 1 - kmin / PF_KT;
+                    }
+                    const int64_t up = scan(cnt), last = __shfl_sync(0xffffffffu, up, 31);
+                    if (rel >= last) {
+                        rel -= last;
+                        continue;
+                    }
+                    const int w = __ffs(__ballot_sync(0xffffffffu, up > rel)) - 1;
+                    if (lane == w) {
+                        PfItem x;
+                        x.e = e; x.b = b0 + at; x.hk = hk; x.mt = m0 + w;
+                        x.off = PF_ITEM - (int)(rel - (up - cnt));
+                        pf_set(p, G, len, x);
+                        sh.item[0] = x;
+                        if (x.off >= len) len = 0;   // nothing but the beginning of an item's cost
+                    }
+                    break;
+                }
+                break;
+            }
         }
-        const uint32_t past = __ballot_sync(0xffffffffu, (int64_t)inc * n_kv > rel);
-        const int at = __ffs(past) - 1;
-        rel -= (int64_t)(__shfl_sync(0xffffffffu, inc - mine, at)) * n_kv;
-        tiles_m = __shfl_sync(0xffffffffu, mine, at);
-        e = kv_check_entry(kv, p.rows, b0 + at);
-        break;
-    }
-    if (tiles_m == 0) return;
-    const int hk = (int)(rel / tiles_m), pr0 = (tiles_m - 1 - (int)(rel % tiles_m)) * PF_M;
-    const int npairs = (int)min((int64_t)e.rows * G - pr0, (int64_t)PF_M);
-    const int all_hi = e.pos0 + pr0 / G, kmax = e.pos0 + (pr0 + npairs - 1) / G;   // the first and last pair's positions
-    const int kmin = p.window > 0 ? max(0, all_hi - p.window + 1) : 0;
-    const int all_lo = p.window > 0 ? max(0, kmax - p.window + 1) : 0;
-    const int tiles = kmax / PF_KT + 1 - kmin / PF_KT;
-    const int ta = kmin / PF_KT + (int)((int64_t)tiles * split / splits);
-    const int n = kmin / PF_KT + (int)((int64_t)tiles * (split + 1) / splits) - ta;   // this CTA's tiles
-
-    if (tid == 0) {
+        len = __reduce_min_sync(0xffffffffu, len);
+        if (lane == 0) {
+            sh.all = all;
+            sh.ctas = ctas;
+            sh.len = len;
+        }
+    } else if (warp == 2 && lane == 0) {
         for (int i = 0; i < PF_RAW; ++i) {
             mbar_init(&sh.raw_full[i], 1);
-            mbar_init(&sh.raw_empty[i], 4);
+            mbar_init(&sh.raw_empty[i], 8);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.k_full[i], 4);
@@ -199,17 +432,26 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
             mbar_init(&sh.v_empty[i], 1);
             mbar_init(&sh.s_full[i], 1);
             mbar_init(&sh.s_empty[i], 4);
+            mbar_init(&sh.p_full[i], 4);
+            mbar_init(&sh.p_empty[i], 1);
+            mbar_init(&sh.o_full[i], 1);
+            mbar_init(&sh.o_empty[i], 4);
+            mbar_init(&sh.ml_full[i], 8);
+            mbar_init(&sh.ml_empty[i], 8);
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q) mbar_init(&sh.m_full[i][q], 1);
         }
+        mbar_init(&sh.part_full, 8);
+        mbar_init(&sh.last_full, 1);
         mbar_init(&sh.q_full, 4);
-        mbar_init(&sh.p_full, 4);
-        mbar_init(&sh.p_empty, 1);
-        mbar_init(&sh.o_full, 1);
-        mbar_init(&sh.o_empty, 8);
-        mbar_init(&sh.fin, 4);
-        sh.abort = 0;
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&sh.q_empty[i], 1);
+            mbar_init(&sh.meta_full[i], 4);
+            mbar_init(&sh.item_full[i], 1);
+            mbar_init(&sh.item_empty[i], PF_ITEM_USERS);
+        }
         fence_mbar_init();
-    }
-    if (warp == 1) {
+    } else if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -218,316 +460,527 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
+    const int len = sh.len;
 
-    if (warp == 0) {
-        // ---------------- copies: a group of 16 positions a lane ----------------
-        const int32_t* pages = kv.table + (int64_t)e.seq * kv.max_pages;
-        const int per = 1 << (kv.page_shift - 4);
-        auto page_of = [&](int i) {
-            const int pos = (ta + i) * PF_KT + 16 * lane;
-            return lane < PF_GROUPS && i < n && pos <= kmax ? pages[pos >> kv.page_shift] : -1;
-        };
-        int id = page_of(0);
-        for (int i = 0; i < n; ++i) {
-            const int st = i % PF_RAW;
-            if (!pf_wait_warp(&sh.raw_empty[st], (i / PF_RAW & 1) ^ 1, sh, kv.err)) break;
-            const uint32_t have = __popc(__ballot_sync(0xffffffffu, id >= 0));
-            if (lane == 0) mbar_arrive_expect_tx(&sh.raw_full[st], have * kv_group_bytes(R));
-            __syncwarp();
-            if (id >= 0) {
-                const int grp = ((ta + i) * PF_KT + 16 * lane) >> 4 & (per - 1);
-                bulk_g2s(smem + st * S::RAW_BYTES + lane * kv_group_bytes(R),
-                         kv.pages + (((int64_t)id * n_kv + hk) * per + grp) * kv_group_bytes(R), kv_group_bytes(R),
-                         &sh.raw_full[st]);
+    // i counts the run's tiles, j its items; a ring's slot and phase follow from them
+    if (warp < PF_W_SOFT) {
+        regs_dec<PF_REGS_ISSUE>();
+        if (warp == 0 && len > 0) {
+            // ---------------- copies: a group of 16 positions a lane ----------------
+            const int per = 1 << (kv.page_shift - 4);
+            PfItem x;
+            int i = 0;
+            bool ok = true;
+#pragma unroll 1
+            for (int j = 0; ok && pf_item(sh, j, x, kv.err); ++j) {
+                const int32_t* pages = kv.table + (int64_t)x.e.seq * kv.max_pages;
+                auto page_of = [&](int t) {
+                    const int pos = (x.ta + t) * PF_KT + 16 * lane;
+                    return lane < PF_GROUPS && t < x.n && pos <= x.kmax ? pages[pos >> kv.page_shift] : -1;
+                };
+                int id = page_of(0);
+#pragma unroll 1
+                for (int t = 0; t < x.n && ok; ++t, ++i) {
+                    const int st = i % PF_RAW;
+                    ok = pf_wait_warp(&sh.raw_empty[st], (i / PF_RAW & 1) ^ 1, kv.err);
+                    if (!ok) break;
+                    const uint32_t have = __popc(__ballot_sync(0xffffffffu, id >= 0));
+                    if (lane == 0) mbar_arrive_expect_tx(&sh.raw_full[st], have * kv_group_bytes(R));
+                    __syncwarp();
+                    if (id >= 0) {
+                        const int grp = ((x.ta + t) * PF_KT + 16 * lane) >> 4 & (per - 1);
+                        bulk_g2s(smem + st * S::RAW_BYTES + lane * kv_group_bytes(R),
+                                 kv.pages + (((int64_t)id * n_kv + x.hk) * per + grp) * kv_group_bytes(R),
+                                 kv_group_bytes(R), &sh.raw_full[st]);
+                    }
+                    id = page_of(t + 1);
+                }
+                pf_item_done(sh, j, lane);
             }
-            id = page_of(i + 1);
-        }
-    } else if (warp == 1) {
-        // ---------------- MMA issue ----------------
-        if (n > 0) {
-            constexpr uint32_t iqk = umma_idesc_f16(PF_M, PF_KT), ipv = umma_idesc_f16(PF_M, HD);
+        } else if (warp == 1 && len > 0) {
+            // ---------------- MMA issue: S = q k ----------------
+            constexpr uint32_t idesc = umma_idesc_f16(PF_M, PF_KT);
             const uint64_t kdesc = umma_desc_k(smem_u32(smem + S::K), S::K_PIECE, 128);
+            PfItem x;
+            int i = 0;
+            bool ok = true;
+#pragma unroll 1
+            for (int j = 0; ok && pf_item(sh, j, x, kv.err); ++j) {
+                ok = pf_wait_warp(&sh.q_full, j & 1, kv.err);
+#pragma unroll 1
+                for (int t = 0; t < x.n && ok; ++t, ++i) {
+                    const int b = i & 1;
+                    ok = pf_wait_warp(&sh.k_full[b], i >> 1 & 1, kv.err) &&
+                         pf_wait_warp(&sh.s_empty[b], (i >> 1 & 1) ^ 1, kv.err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t hi = kdesc + b * (2 * S::K_PART / 16);
+                        const uint32_t d = tmem + PF_T_S + b * PF_KT;
+#pragma unroll
+                        for (int pass = 0; pass < 3; ++pass)
+#pragma unroll
+                            for (int s = 0; s < HD / 16; ++s)
+                                umma_f16_ts(d, tmem + (pass == 0 ? PF_T_QL : PF_T_QH) + 8 * s,
+                                            hi + ((pass == 1 ? S::K_PART : 0) + s * 2 * S::K_PIECE) / 16, idesc, pass + s > 0);
+                        umma_commit(&sh.s_full[b]);
+                        umma_commit(&sh.k_empty[b]);
+                        if (t == x.n - 1) umma_commit(&sh.q_empty[j & 3]);
+                    }
+                    __syncwarp();
+                }
+                pf_item_done(sh, j, lane);
+            }
+        } else if (warp == 2 && len > 0) {
+            // ---------------- MMA issue: O = p v, half of the dims at a time: one is read while the other is made ----------------
+            constexpr uint32_t idesc = umma_idesc_f16(PF_M, HD / 2);
             const uint64_t vdesc = umma_desc_k(smem_u32(smem + S::V), S::V_PIECE, S::V_GROUP);
-            auto qk = [&](int i) -> bool {
-                const int b = i & 1;
-                if (!pf_wait_warp(&sh.k_full[b], i >> 1 & 1, sh, kv.err) ||
-                    !pf_wait_warp(&sh.s_empty[b], (i >> 1 & 1) ^ 1, sh, kv.err))
-                    return false;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint64_t hi = kdesc + b * (2 * S::K_PART / 16);
-                    const uint32_t d = tmem + PF_T_S + b * PF_KT;
-#pragma unroll
-                    for (int pass = 0; pass < 3; ++pass)
-#pragma unroll
-                        for (int s = 0; s < HD / 16; ++s)
-                            umma_f16_ts(d, tmem + (pass == 0 ? PF_T_QL : PF_T_QH) + 8 * s,
-                                        hi + ((pass == 1 ? S::K_PART : 0) + s * 2 * S::K_PIECE) / 16, iqk, pass + s > 0);
-                    umma_commit(&sh.s_full[b]);
-                    umma_commit(&sh.k_empty[b]);
+            PfItem x;
+            int j = 0, tiles = 0;
+            bool ok = true;
+#pragma unroll 1
+            for (int i = 0; ok; ++i) {
+                if (i == tiles) {
+                    if (!pf_item(sh, j, x, kv.err)) break;
+                    tiles += x.n;
+                    pf_item_done(sh, j++, lane);
                 }
-                __syncwarp();
-                return true;
-            };
-            auto pv = [&](int i) -> bool {
                 const int b = i & 1;
-                if (!pf_wait_warp(&sh.p_full, i & 1, sh, kv.err) || !pf_wait_warp(&sh.v_full[b], i >> 1 & 1, sh, kv.err) ||
-                    !pf_wait_warp(&sh.o_empty, (i & 1) ^ 1, sh, kv.err))
-                    return false;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint64_t hi = vdesc + b * (2 * S::V_PART / 16);
+                ok = pf_wait_warp(&sh.p_full[b], i >> 1 & 1, kv.err) && pf_wait_warp(&sh.v_full[b], i >> 1 & 1, kv.err);
+#pragma unroll 1
+                for (int h = 0; h < 2 && ok; ++h) {
+                    ok = pf_wait_warp(&sh.o_empty[h], (i & 1) ^ 1, kv.err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t hi = vdesc + b * (2 * S::V_PART / 16) + h * (HD / 16 * S::V_GROUP / 16);
+                        const uint32_t tp = tmem + PF_T_P + b * PF_KT, to = tmem + PF_T_O + h * (HD / 2);
 #pragma unroll
-                    for (int pass = 0; pass < 3; ++pass)
+                        for (int pass = 0; pass < 3; ++pass)
 #pragma unroll
-                        for (int s = 0; s < PF_KT / 16; ++s)
-                            umma_f16_ts(tmem + PF_T_O, tmem + (pass == 0 ? PF_T_PL : PF_T_PH) + 8 * s,
-                                        hi + ((pass == 1 ? S::V_PART : 0) + s * 2 * S::V_PIECE) / 16, ipv, pass + s > 0);
-                    umma_commit(&sh.o_full);
-                    umma_commit(&sh.v_empty[b]);
-                    umma_commit(&sh.p_empty);
+                            for (int s = 0; s < PF_KT / 16; ++s)
+                                umma_f16_ts(to, tp + (pass == 0 ? PF_KT / 2 : 0) + 8 * s,
+                                            hi + ((pass == 1 ? S::V_PART : 0) + s * 2 * S::V_PIECE) / 16, idesc, pass + s > 0);
+                        umma_commit(&sh.o_full[h]);
+                        if (h == 1) {
+                            umma_commit(&sh.v_empty[b]);
+                            umma_commit(&sh.p_empty[b]);
+                        }
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
-                return true;
-            };
-            bool ok = pf_wait_warp(&sh.q_full, 0, sh, kv.err) && qk(0);
-            for (int i = 0; i < n && ok; ++i) ok = (i + 1 >= n || qk(i + 1)) && pv(i);
+            }
+        } else if (warp == 3 && len > 0) {
+            // ---------------- the run's items, and their q rows to L2 ----------------
+            PfItem x = sh.item[0];
+            bool more = true;
+#pragma unroll 1
+            for (int j = 0; more; ++j) {
+                if (j > 0) {
+                    more = pf_next(p, G, len, x);
+                    if (!pf_wait_warp(&sh.item_empty[j & 3], (j >> 2 & 1) ^ 1, kv.err)) break;
+                    if (!more) x.n = 0;
+                    if (lane == 0) sh.item[j & 3] = x;
+                    __syncwarp();
+                }
+                if (lane == 0) mbar_arrive(&sh.item_full[j & 3]);
+                if (j == 0 || !more) continue;
+#pragma unroll 1
+                for (int r = lane; r < x.npairs; r += 32) {
+                    int64_t at;
+                    pf_q_at<R>(p, x, G, r, at);
+#pragma unroll
+                    for (int d = 0; d < HD; d += 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.q + at + d));
+                }
+            }
         }
         __syncwarp();
     } else if (warp < PF_W_SUM) {
-        // ---------------- softmax: thread = row 32 (warp % 4) + lane ----------------
-        const int r = 32 * (warp & 3) + lane;
-        const uint32_t tq = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-        const int pi = pr0 + min(r, npairs - 1), j = pi / G;   // missing pairs repeat the last one
-        const int qpos = e.pos0 + j, qlo = p.window > 0 ? qpos - p.window + 1 : 0;
-        float sfac;
-        {   // q: two fp16 parts times a power of two, amax * f in [2^13, 2^14)
-            const float* qr = p.q + (int64_t)(e.row0 + j) * p.ldq + (int64_t)(hk * G + pi - j * G) * HD;
-            float amax = 0.0f;
-            for (int d = 0; d < HD; d += 4) {
-                const float4 x = *reinterpret_cast<const float4*>(qr + d);
-                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-            }
-            const int fe = min(253, max(1, 267 - (int)(__float_as_uint(amax) >> 23)));
-            const float f = copysignf(__uint_as_float((uint32_t)fe << 23), p.scale);
-            // (never 0: a masked score is -inf times it)
-            sfac = fmaxf(fabsf(p.scale) * 1.44269504088896341f * __uint_as_float((uint32_t)(254 - fe) << 23), 1e-36f);
-            for (int d = 0; d < HD; d += 16) {   // dims (0, 4 | 1, 5 | 2, 6 | 3, 7) of each 8, as K's are unpacked
-                uint32_t hi[8], lo[8];
+        // ---------------- softmax: thread = row, a warpgroup every other tile ----------------
+        regs_inc<PF_REGS_SOFT>();
+        const int w = warp & 3, r = 32 * w + lane, b = (warp - PF_W_SOFT) / 4;
+        const uint32_t tq = tmem + ((uint32_t)(32 * w) << 16), ts = tq + PF_T_S + b * PF_KT, tp = tq + PF_T_P + b * PF_KT;
+        if (len > 0) {
+            PfItem x;
+            int i = 0;
+            bool ok = true;
+#pragma unroll 1
+            for (int j = 0; ok && pf_item(sh, j, x, kv.err); ++j) {
+                const int pi = x.pr0 + min(r, x.npairs - 1);   // missing pairs repeat the last one
+                const int qpos = x.e.pos0 + pi / G, qlo = p.window > 0 ? qpos - p.window + 1 : 0;
+                float m = -INFINITY, l = 0.0f, sfac = 0.0f;   // of this warpgroup's tiles
+                bool fresh = true;
+#pragma unroll 1
+                for (int t = 0; t < x.n && ok; ++t, ++i) {
+                    if ((i & 1) != b) continue;
+                    ok = pf_wait_warp(&sh.s_full[b], i >> 1 & 1, kv.err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (fresh) sfac = sh.sfac[j & 3][r];
+                    fresh = false;
+                    const float up = sh.unscale[i & 3], f = sfac * up;
+                    const int k0 = (x.ta + t) * PF_KT;
+                    const bool full = k0 >= x.all_lo && k0 + PF_KT - 1 <= x.all_hi;   // no key is masked for any row
+                    // the row's keys, as bits from k0 on
+                    const uint64_t see = full ? ~0ull
+                                              : (~0ull >> (63 - min(63, max(0, qpos - k0)))) & (~0ull << min(63, max(0, qlo - k0))) &
+                                                    (qpos < k0 || qlo > k0 + 63 ? 0 : ~0ull);
+                    // a NaN among V's scales: the rows that see its key become NaN, the others do not (the unpacked value is 0)
+                    const uint64_t bad = sh.poison[i & 3];
+                    if (bad & see) l = __uint_as_float(0x7fffffffu);
+                    float mx = -INFINITY;
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        float v[32];
+                        tmem_ld32(ts + 32 * h, v);
+                        tmem_ld_wait();
+                        if (!full) {
+                            const uint32_t s32 = (uint32_t)(see >> 32 * h);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float4 x = *reinterpret_cast<const float4*>(qr + d + 8 * h);
-                    const float4 y = *reinterpret_cast<const float4*>(qr + d + 8 * h + 4);
-                    split_half2(x.x * f, y.x * f, hi[4 * h], lo[4 * h]);
-                    split_half2(x.y * f, y.y * f, hi[4 * h + 1], lo[4 * h + 1]);
-                    split_half2(x.z * f, y.z * f, hi[4 * h + 2], lo[4 * h + 2]);
-                    split_half2(x.w * f, y.w * f, hi[4 * h + 3], lo[4 * h + 3]);
-                }
-                tmem_st8(tq + PF_T_QH + d / 2, hi);
-                tmem_st8(tq + PF_T_QL + d / 2, lo);
-            }
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.q_full);
-        }
-        float m = -INFINITY, l = 0.0f;
-        for (int i = 0; i < n; ++i) {
-            const int b = i & 1;
-            if (!pf_wait_warp(&sh.s_full[b], i >> 1 & 1, sh, kv.err)) break;
-            tc_fence_after();
-            float v[2][32];
-            tmem_ld32(tq + PF_T_S + b * PF_KT, v[0]);
-            tmem_ld32(tq + PF_T_S + b * PF_KT + 32, v[1]);
-            tmem_ld_wait();
-            tc_fence_before();
-            const float up = sh.unscale[i & 3], f = sfac * up;
-            const int k0 = (ta + i) * PF_KT;
-            const bool full = k0 >= all_lo && k0 + PF_KT - 1 <= all_hi;   // no key is masked for any row
-            if (!full) {
+                            for (int c = 0; c < 32; ++c)
+                                if (!(s32 >> c & 1)) v[c] = -INFINITY;
+                        }
+                        float a0 = v[0], a1 = v[1];
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (k0 + 32 * h + c > qpos || k0 + 32 * h + c < qlo) v[h][c] = -INFINITY;
-            }
-            // a NaN among V's scales: the rows that see its key become NaN, the others do not (the unpacked value is 0)
-#pragma unroll
-            for (int g = 0; g < PF_GROUPS; ++g) {
-                uint32_t bad = sh.poison[i & 3][g];
-                for (; bad; bad &= bad - 1) {
-                    const int key = k0 + 16 * g + __ffs(bad) - 1;
-                    if (key <= qpos && key >= qlo) l = __uint_as_float(0x7fffffffu);
-                }
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.s_empty[b]);
-            float mx[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], v[h][c]);
-            const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f);
-            const float corr = mn == m ? 1.0f : ex2(m - mn);   // m = -inf: 0
-            m = mn;
-            const float mref = m == -INFINITY ? 0.0f : PF_PLOG2 - m;
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (!pf_wait_warp(&sh.p_empty, (i & 1) ^ 1, sh, kv.err)) break;   // and corr of two tiles before is read
-            tc_fence_after();
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int c = 0; c < 32; c += 16) {
-                    uint32_t hi[8], lo[8];
-#pragma unroll
-                    for (int x = 0; x < 16; x += 2) {
-                        const float p0 = ex2(fmaf(v[h][c + x], f, mref)), p1 = ex2(fmaf(v[h][c + x + 1], f, mref));
-                        sum[x & 2] += p0;
-                        sum[(x & 2) + 1] += p1;
-                        split_half2(p0 * up, p1 * up, hi[x / 2], lo[x / 2]);
+                        for (int c = 2; c < 32; c += 2) {
+                            a0 = fmaxf(a0, v[c]);
+                            a1 = fmaxf(a1, v[c + 1]);
+                        }
+                        mx = fmaxf(mx, fmaxf(a0, a1));
                     }
-                    tmem_st8(tq + PF_T_PH + 16 * h + c / 2, hi);
-                    tmem_st8(tq + PF_T_PL + 16 * h + c / 2, lo);
+                    // the running maximum passes from one warpgroup's tile to the other's
+                    if (i > 0) ok = pf_wait_warp(&sh.m_full[b ^ 1][w], (i - 1) >> 1 & 1, kv.err);
+                    const float before = t == 0 ? -INFINITY : sh.m[b ^ 1][r];
+                    const float mn = fmaxf(before, mx * f);
+                    sh.m[b][r] = mn;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.m_full[b][w]);
+                    const float corr = mn == before ? 1.0f : ex2(before - mn);   // before = -inf: 0
+                    l *= mn == m ? 1.0f : ex2(m - mn);
+                    m = mn;
+                    // p times 2^9, and 2^4 more where the values are taken times 2^-4
+                    const float mref = m == -INFINITY ? 0.0f : PF_PLOG2 + (up == 1.0f ? 0.0f : 4.0f) - m;
+                    const uint64_t f2 = f2_packf(f, f), mref2 = f2_packf(mref, mref), minus = f2_packf(-1.0f, -1.0f);
+                    ok = ok && pf_wait_warp(&sh.p_empty[b], (i >> 1 & 1) ^ 1, kv.err);   // and corr of four tiles before is read
+                    if (!ok) break;
+                    tc_fence_after();
+                    uint64_t sum = f2_packf(0.0f, 0.0f);
+#pragma unroll 1
+                    for (int h = 0; h < 4; ++h) {
+                        float v[16];
+                        tmem_ld16(ts + 16 * h, v);
+                        tmem_ld_wait();
+                        if (h == 3) {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&sh.s_empty[b]);
+                        }
+                        if (!full) {
+                            const uint32_t s16 = (uint32_t)(see >> 16 * h);
+#pragma unroll
+                            for (int c = 0; c < 16; ++c)
+                                if (!(s16 >> c & 1)) v[c] = -INFINITY;
+                        }
+                        uint32_t hi[8], lo[8];
+#pragma unroll
+                        for (int y = 0; y < 16; y += 2) {
+                            const float2 a = f2_float2(f2_fma(f2_packf(v[y], v[y + 1]), f2, mref2));
+                            const float p0 = ex2(a.x), p1 = ex2(a.y);
+                            const uint64_t pp = f2_packf(p0, p1);
+                            sum = f2_add(sum, pp);
+                            const __half2 ph = __floats2half2_rn(p0, p1);
+                            const float2 pf = __half22float2(ph);
+                            hi[y / 2] = *reinterpret_cast<const uint32_t*>(&ph);
+                            const float2 rest = f2_float2(f2_fma(f2_packf(pf.x, pf.y), minus, pp));
+                            lo[y / 2] = pack_half2(rest.x, rest.y);
+                        }
+                        tmem_st8(tp + 8 * h, hi);
+                        tmem_st8(tp + PF_KT / 2 + 8 * h, lo);
+                    }
+                    const float2 sf = f2_float2(sum);
+                    l = fmaf(sf.x + sf.y, up == 1.0f ? 1.0f : 0.0625f, l);
+                    sh.corr[i & 3][r] = corr;
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.p_full[b]);
                 }
-            l = l * corr + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-            sh.corr[b][r] = corr;
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.p_full);
+                ok = ok && pf_wait_warp(&sh.ml_empty[j & 1], (j >> 1 & 1) ^ 1, kv.err);
+                sh.ml[j & 1][b][r] = make_float2(m, l);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.ml_full[j & 1]);
+                pf_item_done(sh, j, lane);
+            }
         }
-        sh.m[r] = m;
-        sh.l[r] = l;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.fin);
     } else if (warp < PF_W_UNPACK) {
         // ---------------- O: thread = row, half of its dims ----------------
+        regs_inc<PF_REGS_SUM>();
         constexpr int NC = HD / 2;
-        const int r = 32 * (warp & 3) + lane, c0 = (warp - PF_W_SUM) / 4 * NC;
-        const uint32_t to = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + PF_T_O + c0;
-        float o[NC];
+        const int w8 = warp - PF_W_SUM, w = warp & 3, r = 32 * w + lane, c0 = w8 / 4 * NC;
+        const uint32_t to = tmem + ((uint32_t)(32 * w) << 16) + PF_T_O + c0;
+        float* stage = reinterpret_cast<float*>(smem + S::OSTAGE) + w8 * 32 * PF_OS;
+        if (len > 0) {
+            PfItem x;
+            int i = 0, cuts = 0;
+            bool ok = true;
+#pragma unroll 1
+            for (int j = 0; ok && pf_item(sh, j, x, kv.err); ++j) {
+                uint64_t o[NC / 2];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) o[c] = 0.0f;
-        bool ok = true;
-        for (int i = 0; i < n && ok; ++i) {
-            ok = pf_wait_warp(&sh.o_full, i & 1, sh, kv.err);
-            if (!ok) break;
-            tc_fence_after();
-            const float corr = sh.corr[i & 1][r];
+                for (int c = 0; c < NC / 2; ++c) o[c] = 0;
+#pragma unroll 1
+                for (int t = 0; t < x.n && ok; ++t, ++i) {
+                    ok = pf_wait_warp(&sh.o_full[w8 / 4], i & 1, kv.err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const float corr = sh.corr[i & 3][r];
+                    const uint64_t corr2 = f2_packf(corr, corr);
 #pragma unroll
-            for (int h = 0; h < NC; h += 32) {
-                float t[32];
-                tmem_ld32(to + h, t);
-                tmem_ld_wait();
+                    for (int h = 0; h < NC; h += 16) {
+                        float v[16];
+                        tmem_ld16(to + h, v);
+                        tmem_ld_wait();
 #pragma unroll
-                for (int c = 0; c < 32; ++c) o[h + c] = fmaf(o[h + c], corr, t[c]);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.o_empty);
-        }
-        ok = ok && pf_wait_warp(&sh.fin, 0, sh, kv.err);
-        if (ok && r < npairs) {
-            const int pi = pr0 + r, j = pi / G;
-            float* dst = splits == 1 ? p.out + (int64_t)(e.row0 + j) * p.ldo + (int64_t)(hk * G + pi - j * G) * HD + c0
-                                     : reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + KV_COUNTER_BYTES) +
-                                           ((item * splits + split) * PF_M + r) * (HD + 4) + c0;
-            const float f = splits == 1 ? 1.0f / sh.l[r] : 1.0f;
-#pragma unroll
-            for (int c = 0; c < NC; c += 4)
-                __stcg(reinterpret_cast<float4*>(dst + c), make_float4(o[c] * f, o[c + 1] * f, o[c + 2] * f, o[c + 3] * f));
-            if (splits > 1 && c0 == 0) __stcg(reinterpret_cast<float2*>(dst + HD), make_float2(sh.m[r], sh.l[r]));
-        }
-    } else {
-        // ---------------- unpacking: warp = group of the tile ----------------
-        const int grp = warp - PF_W_UNPACK, g = lane >> 2, q = lane & 3;
-        const uint32_t base = p.code_base;
-        for (int i = 0; i < n; ++i) {
-            const int b = i & 1, st = i % PF_RAW;
-            const uint8_t* tile = smem + st * S::RAW_BYTES;
-            const uint8_t* raw = tile + grp * kv_group_bytes(R);
-            const int k0 = (ta + i) * PF_KT;
-            if (!pf_wait_warp(&sh.raw_full[st], i / PF_RAW & 1, sh, kv.err)) break;
-            if (!pf_wait_warp(&sh.k_empty[b], (i >> 1 & 1) ^ 1, sh, kv.err)) break;
-            // the largest scale of the tile's live groups (as fp16 bits): above 8188 its values are taken times 2^-4,
-            // so that d (c - 8) stays in fp16's range; above infinity some are NaN
-            uint32_t top = 0;
-#pragma unroll
-            for (int x = 0; x < PF_GROUPS; ++x)
-                if (k0 + 16 * x <= kmax)
-#pragma unroll
-                    for (int w = lane; w < 16 * R; w += 32)
-                        top = __vmaxu2(top, reinterpret_cast<const uint32_t*>(tile + x * kv_group_bytes(R) + 512 * R)[w] & 0x7FFF7FFFu);
-            top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
-            const bool big = top > 0x6FFFu;
-            uint32_t nan = 0;
-            if (top > 0x7C00u && k0 + 16 * grp <= kmax) {
-                bool mine = false;   // lane = position
-#pragma unroll
-                for (int x = 0; x < R; ++x)
-                    mine |= (reinterpret_cast<const uint16_t*>(raw + 544 * R)[kv_vscale(R, lane & 15, x)] & 0x7FFFu) > 0x7C00u;
-                nan = __ballot_sync(0xffffffffu, mine) & 0xFFFFu;
-            }
-            if (lane == 0) {
-                sh.poison[i & 3][grp] = nan;
-                if (grp == 0) sh.unscale[i & 3] = big ? 16.0f : 1.0f;
-            }
-            uint8_t* kd = smem + S::K + b * 2 * S::K_PART;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {   // key 8 u + g, dims 32 x + 8 q .. + 7
-                uint32_t w[R];
-                __half d[R];
-                load_words<R>(w, raw, u, lane);
-                load_kscales<R>(d, raw + 512 * R, 8 * u + g);
-#pragma unroll
-                for (int x = 0; x < R; ++x) {
-                    __half2 dd = __half2half2(d[x]);
-                    uint32_t d2 = *reinterpret_cast<uint32_t*>(&dd), c[4];
-                    if (big) d2 = mul_h2(d2, 0x2C002C00u);
-                    unpack(c, w[x], base);
-                    uint4 hi, lo;
-                    hi.x = mul_h2(c[0], d2); lo.x = fma_h2(c[0], d2, neg_h2(hi.x));
-                    hi.y = mul_h2(c[1], d2); lo.y = fma_h2(c[1], d2, neg_h2(hi.y));
-                    hi.z = mul_h2(c[2], d2); lo.z = fma_h2(c[2], d2, neg_h2(hi.z));
-                    hi.w = mul_h2(c[3], d2); lo.w = fma_h2(c[3], d2, neg_h2(hi.w));
-                    uint8_t* at = kd + (4 * x + q) * S::K_PIECE + (16 * grp + 8 * u + g) * 16;
-                    *reinterpret_cast<uint4*>(at) = hi;
-                    *reinterpret_cast<uint4*>(at + S::K_PART) = lo;
+                        for (int c = 0; c < 16; c += 2) o[(h + c) / 2] = f2_fma(o[(h + c) / 2], corr2, f2_packf(v[c], v[c + 1]));
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.o_empty[w8 / 4]);
                 }
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.k_full[b]);
-            if (!pf_wait_warp(&sh.v_empty[b], (i >> 1 & 1) ^ 1, sh, kv.err)) break;
-            uint8_t* vd = smem + S::V + b * 2 * S::V_PART;
+                // the item's end
+                ok = ok && pf_wait_warp(&sh.ml_full[j & 1], j >> 1 & 1, kv.err);
+                if (!ok) break;
+                const float2 ml0 = sh.ml[j & 1][0][r], ml1 = sh.ml[j & 1][1][r];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.ml_empty[j & 1]);
+                const float m = fmaxf(ml0.x, ml1.x);
+                const float l = ml0.y * (ml0.x == -INFINITY ? 0.0f : ex2(ml0.x - m)) +
+                                ml1.y * (ml1.x == -INFINITY ? 0.0f : ex2(ml1.x - m));
+                const int pi = x.pr0 + min(r, x.npairs - 1), qr = pi / G;
+                const int64_t row_at = (int64_t)(x.e.row0 + qr) * p.ldo + (int64_t)(x.hk * G + pi - qr * G) * HD + c0;
+                // 16 dims of the warp's rows go to `out` by way of shared memory: 64 bytes of 8 rows at a time
+                auto write = [&](int c, const float (&v)[16]) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {   // keys 8 u + 2 q, + 1, dims 32 x + 4 g .. + 3
-                uint32_t w[R], d[R];
-                load_words<R>(w, raw + 256 * R, u, lane);
-                load_scales<R>(d, raw + 544 * R, u, q);
-                // keys that no row sees may hold anything: 0
-                const int key = 8 * u + 2 * q, pos = k0 + 16 * grp + key;
-                uint32_t live = (pos > kmax || pos < kmin || (nan >> key & 1) ? 0u : 0xFFFFu) |
-                                (pos + 1 > kmax || pos + 1 < kmin || (nan >> key & 2) ? 0u : 0xFFFF0000u);
+                    for (int k = 0; k < 16; k += 4)
+                        *reinterpret_cast<float4*>(stage + lane * PF_OS + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                    __syncwarp();
 #pragma unroll
-                for (int x = 0; x < R; ++x) {
-                    uint32_t d2 = d[x] & live, c[4];
-                    if (big) d2 = mul_h2(d2, 0x2C002C00u);
-                    unpack(c, w[x], base);
+                    for (int k = 0; k < 32; k += 8) {
+                        const int row = k + (lane >> 2);
+                        const int64_t at = __shfl_sync(0xffffffffu, row_at, row);
+                        const float4 y = *reinterpret_cast<const float4*>(stage + row * PF_OS + 4 * (lane & 3));
+                        if (32 * w + row < x.npairs) *reinterpret_cast<float4*>(p.out + at + c + 4 * (lane & 3)) = y;
+                    }
+                    __syncwarp();
+                };
+                if (x.off >= 0 && x.off + x.cnt <= len) {
+                    const float f = 1.0f / l;
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        const uint32_t hi = mul_h2(c[y], d2), lo = fma_h2(c[y], d2, neg_h2(hi));
-                        uint8_t* at = vd + (2 * grp + u) * S::V_PIECE + (4 * x + (g >> 1)) * S::V_GROUP + (4 * (g & 1) + y) * 16 + 4 * q;
-                        *reinterpret_cast<uint32_t*>(at) = hi;
-                        *reinterpret_cast<uint32_t*>(at + S::V_PART) = lo;
+                    for (int c = 0; c < NC; c += 16) {
+                        float v[16];
+#pragma unroll
+                        for (int k = 0; k < 16; k += 2) {
+                            const float2 y = f2_float2(o[(c + k) / 2]);
+                            v[k] = y.x * f;
+                            v[k + 1] = y.y * f;
+                        }
+                        write(c, v);
+                    }
+                } else {
+                    // others have parts of it: the last of its CTAs to arrive joins them.  A CTA keeps at most two: of an
+                    // item that begins before its run, and of one that ends behind it.
+                    const int64_t begin = sh.all * blockIdx.x / sh.ctas + x.off;
+                    const int cta0 = (int)(((begin + 1) * sh.ctas - 1) / sh.all);
+                    const int parts = (int)(((begin + x.cnt) * sh.ctas - 1) / sh.all) - cta0 + 1;
+                    int* counter = reinterpret_cast<int*>(p.workspace) + cta0;
+                    float* ws = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + KV_COUNTER_BYTES);
+                    auto part = [&](int k) { return ws + (int64_t)(2 * (cta0 + k) + (k == 0)) * (PF_M * (HD + 4)); };
+                    float* mine = part(blockIdx.x - cta0);
+#pragma unroll
+                    for (int c = 0; c < NC; c += 4) {
+                        const float2 y0 = f2_float2(o[c / 2]), y1 = f2_float2(o[c / 2 + 1]);
+                        __stcg(reinterpret_cast<float4*>(mine) + (w8 * (NC / 4) + c / 4) * 32 + lane,
+                               make_float4(y0.x, y0.y, y1.x, y1.y));
+                    }
+                    if (c0 == 0) __stcg(reinterpret_cast<float2*>(mine + PF_M * HD) + r, make_float2(m, l));
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.part_full);
+                    if (w8 == 0) {
+                        ok = pf_wait_warp(&sh.part_full, cuts & 1, kv.err);
+                        if (!ok) break;
+                        if (lane == 0) {
+                            __threadfence();
+                            const int last = atomicAdd(counter, 1) == parts - 1;
+                            __threadfence();
+                            sh.last = last;
+                            if (last) *counter = 0;
+                            mbar_arrive(&sh.last_full);
+                        }
+                        __syncwarp();
+                    }
+                    ok = pf_wait_warp(&sh.last_full, cuts & 1, kv.err);
+                    if (!ok) break;
+                    ++cuts;
+                    if (sh.last) {
+                        float M = -INFINITY, L = 0.0f;
+#pragma unroll 1
+                        for (int k = 0; k < parts; ++k)
+                            M = fmaxf(M, __ldcg(reinterpret_cast<const float2*>(part(k) + PF_M * HD) + r).x);
+#pragma unroll 1
+                        for (int k = 0; k < parts; ++k) {
+                            const float2 y = __ldcg(reinterpret_cast<const float2*>(part(k) + PF_M * HD) + r);
+                            L += y.y * (y.x == -INFINITY ? 0.0f : ex2(y.x - M));
+                        }
+                        const float inv = 1.0f / L;
+#pragma unroll 1
+                        for (int c = 0; c < NC; c += 16) {
+                            float v[16];
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) v[k] = 0.0f;
+#pragma unroll 2
+                            for (int k = 0; k < parts; ++k) {
+                                const float my = __ldcg(reinterpret_cast<const float2*>(part(k) + PF_M * HD) + r).x;
+                                const float a = my == -INFINITY ? 0.0f : ex2(my - M) * inv;
+#pragma unroll
+                                for (int y = 0; y < 4; ++y) {
+                                    const float4 z =
+                                        __ldcg(reinterpret_cast<const float4*>(part(k)) + (w8 * (NC / 4) + c / 4 + y) * 32 + lane);
+                                    v[4 * y] += a * z.x;
+                                    v[4 * y + 1] += a * z.y;
+                                    v[4 * y + 2] += a * z.z;
+                                    v[4 * y + 3] += a * z.w;
+                                }
+                            }
+                            write(c, v);
+                        }
                     }
                 }
+                pf_item_done(sh, j, lane);
             }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&sh.v_full[b]);
-                mbar_arrive(&sh.raw_empty[st]);
+        }
+    } else {
+        // ---------------- unpacking: warp = group of the tile, a warpgroup for K and q, one for V ----------------
+        regs_dec<PF_REGS_UNPACK>();
+        const int w = warp & 3, g = lane >> 2, q = lane & 3;
+        const bool is_k = warp < PF_W_UNPACK + 4;
+        const uint32_t base = p.code_base;
+        if (len > 0) {
+            PfItem x;
+            int i = 0;
+            bool ok = true;
+#pragma unroll 1
+            for (int j = 0; ok && pf_item(sh, j, x, kv.err); ++j) {
+                if (is_k) pf_q_max<R>(p, sh, x, G, w, lane);
+#pragma unroll 1
+                for (int t = 0; t < x.n; ++t, ++i) {
+                    const int b = i & 1, st = i % PF_RAW;
+                    const uint8_t* tile = smem + st * S::RAW_BYTES;
+                    const uint8_t* raw = tile + w * kv_group_bytes(R);
+                    const int k0 = (x.ta + t) * PF_KT;
+                    ok = pf_wait_warp(&sh.raw_full[st], i / PF_RAW & 1, kv.err);
+                    if (!ok) break;
+                    if (is_k) {
+                        // the largest scale of the tile's live groups (as fp16 bits): above 8188 its values are taken times
+                        // 2^-4, so that d (c - 8) stays in fp16's range; above infinity some are NaN
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int y = 0; y < PF_GROUPS; ++y)
+                            if (k0 + 16 * y <= x.kmax)
+#pragma unroll
+                                for (int z = lane; z < 16 * R; z += 32)
+                                    top = __vmaxu2(top, reinterpret_cast<const uint32_t*>(tile + y * kv_group_bytes(R) + 512 * R)[z] &
+                                                            0x7FFF7FFFu);
+                        top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
+                        const bool big = top > 0x6FFFu;
+                        uint32_t nan = 0;
+                        if (top > 0x7C00u && k0 + 16 * w <= x.kmax) {
+                            bool mine = false;   // lane = position
+#pragma unroll
+                            for (int y = 0; y < R; ++y)
+                                mine |= (reinterpret_cast<const uint16_t*>(raw + 544 * R)[kv_vscale(R, lane & 15, y)] & 0x7FFFu) > 0x7C00u;
+                            nan = __ballot_sync(0xffffffffu, mine) & 0xFFFFu;
+                        }
+                        ok = pf_wait_warp(&sh.k_empty[b], (i >> 1 & 1) ^ 1, kv.err);
+                        if (!ok) break;
+                        if (lane == 0) {
+                            reinterpret_cast<uint16_t*>(&sh.poison[i & 3])[w] = (uint16_t)nan;
+                            if (w == 0) sh.unscale[i & 3] = big ? 16.0f : 1.0f;
+                            mbar_arrive(&sh.meta_full[i & 3]);
+                        }
+                        const uint32_t shrink = big ? 0x2C002C00u : 0x3C003C00u;   // 2^-4 or 1
+                        uint8_t* kd = smem + S::K + b * 2 * S::K_PART;
+#pragma unroll 1
+                        for (int u = 0; u < 2; ++u) {   // key 8 u + g, dims 32 y + 8 q .. + 7
+                            uint32_t c4[R];
+                            __half d[R];
+                            load_words<R>(c4, raw, u, lane);
+                            load_kscales<R>(d, raw + 512 * R, 8 * u + g);
+#pragma unroll
+                            for (int y = 0; y < R; ++y) {
+                                __half2 dd = __half2half2(d[y]);
+                                uint32_t d2 = *reinterpret_cast<uint32_t*>(&dd), c[4];
+                                d2 = mul_h2(d2, shrink);
+                                unpack(c, c4[y], base);
+                                uint4 hi, lo;
+                                hi.x = mul_h2(c[0], d2); lo.x = fma_h2(c[0], d2, neg_h2(hi.x));
+                                hi.y = mul_h2(c[1], d2); lo.y = fma_h2(c[1], d2, neg_h2(hi.y));
+                                hi.z = mul_h2(c[2], d2); lo.z = fma_h2(c[2], d2, neg_h2(hi.z));
+                                hi.w = mul_h2(c[3], d2); lo.w = fma_h2(c[3], d2, neg_h2(hi.w));
+                                uint8_t* at = kd + (4 * y + q) * S::K_PIECE + (16 * w + 8 * u + g) * 16;
+                                *reinterpret_cast<uint4*>(at) = hi;
+                                *reinterpret_cast<uint4*>(at + S::K_PART) = lo;
+                            }
+                        }
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(&sh.k_full[b]);
+                            mbar_arrive(&sh.raw_empty[st]);
+                        }
+                        if (t == 0)   // behind the first tile's K, which does not wait for the last item's products
+                            ok = pf_q_store<R>(p, sh, reinterpret_cast<float*>(smem + S::QSTAGE), tmem, x, G, j, w, lane);
+                        if (!ok) break;
+                    } else {
+                        // (K's warps are at most the packed tiles in flight ahead: unscale and poison are still this tile's)
+                        ok = pf_wait_warp(&sh.meta_full[i & 3], i >> 2 & 1, kv.err) &&
+                             pf_wait_warp(&sh.v_empty[b], (i >> 1 & 1) ^ 1, kv.err);
+                        if (!ok) break;
+                        const uint32_t shrink = sh.unscale[i & 3] != 1.0f ? 0x2C002C00u : 0x3C003C00u;   // 2^-4 or 1
+                        const uint32_t nan = reinterpret_cast<const uint16_t*>(&sh.poison[i & 3])[w];
+                        uint8_t* vd = smem + S::V + b * 2 * S::V_PART;
+#pragma unroll 1
+                        for (int u = 0; u < 2; ++u) {   // keys 8 u + 2 q, + 1, dims 32 y + 4 g .. + 3
+                            uint32_t c4[R], d[R];
+                            load_words<R>(c4, raw + 256 * R, u, lane);
+                            load_scales<R>(d, raw + 544 * R, u, q);
+                            // keys that no row sees may hold anything: 0
+                            const int key = 8 * u + 2 * q, pos = k0 + 16 * w + key;
+                            const uint32_t live = (pos > x.kmax || pos < x.kmin || (nan >> key & 1) ? 0u : 0xFFFFu) |
+                                                  (pos + 1 > x.kmax || pos + 1 < x.kmin || (nan >> key & 2) ? 0u : 0xFFFF0000u);
+#pragma unroll
+                            for (int y = 0; y < R; ++y) {
+                                uint32_t d2 = d[y] & live, c[4];
+                                d2 = mul_h2(d2, shrink);
+                                unpack(c, c4[y], base);
+#pragma unroll
+                                for (int z = 0; z < 4; ++z) {
+                                    const uint32_t hi = mul_h2(c[z], d2), lo = fma_h2(c[z], d2, neg_h2(hi));
+                                    uint8_t* at = vd + (2 * w + u) * S::V_PIECE + (4 * y + (g >> 1)) * S::V_GROUP +
+                                                  (4 * (g & 1) + z) * 16 + 4 * q;
+                                    *reinterpret_cast<uint32_t*>(at) = hi;
+                                    *reinterpret_cast<uint32_t*>(at + S::V_PART) = lo;
+                                }
+                            }
+                        }
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(&sh.v_full[b]);
+                            mbar_arrive(&sh.raw_empty[st]);
+                        }
+                    }
+                }
+                pf_item_done(sh, j, lane);
             }
         }
     }
@@ -537,38 +990,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
-    if (splits == 1 || sh.abort) return;
-
-    // ---- a split item: the last CTA to arrive joins its parts
-    int* counters = reinterpret_cast<int*>(p.workspace);
-    if (tid == 0) {
-        __threadfence();
-        sh.last = atomicAdd(&counters[item], 1) == splits - 1;
-        __threadfence();
-    }
-    __syncthreads();
-    if (!sh.last) return;
-    const float* parts = reinterpret_cast<const float*>(static_cast<const uint8_t*>(p.workspace) + KV_COUNTER_BYTES) +
-                         item * splits * PF_M * (HD + 4);
-    for (int x = tid; x < npairs * (HD / 4); x += PF_THREADS) {
-        const int r = x / (HD / 4), d = x % (HD / 4) * 4;
-        auto part = [&](int s) { return parts + ((int64_t)s * PF_M + r) * (HD + 4); };
-        float M = -INFINITY, L = 0.0f;
-        for (int s = 0; s < splits; ++s) M = fmaxf(M, __ldcg(part(s) + HD));
-        float4 a = make_float4(0, 0, 0, 0);
-        for (int s = 0; s < splits; ++s) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part(s) + HD));
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(part(s) + d));
-            const float w = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
-            L += w * ml.y;
-            a.x += w * v.x; a.y += w * v.y; a.z += w * v.z; a.w += w * v.w;
-        }
-        const int pi = pr0 + r, j = pi / G;
-        const float inv = 1.0f / L;
-        *reinterpret_cast<float4*>(p.out + (int64_t)(e.row0 + j) * p.ldo + (int64_t)(hk * G + pi - j * G) * HD + d) =
-            make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-    }
-    if (tid == 0) counters[item] = 0;
 }
 
 template <int R>
@@ -581,15 +1002,19 @@ int prefill_r(const KvAttendParams& p, cudaStream_t s) {
     {
         std::lock_guard<std::mutex> lk(mu);
         BREW_CUDA(smem_attr_per_device((const void*)kv_prefill_kernel<R>, smem, &done));
+        static bool checked = false;
+        // the warpgroups' shares of the registers come out of what the block is launched with
+        if (!checked) {
+            cudaFuncAttributes a;
+            BREW_CUDA(cudaFuncGetAttributes(&a, (const void*)kv_prefill_kernel<R>));
+            BREW_CHECK(a.numRegs >= PF_REGS, BREW_ERR_CUDA, "the prompt attention kernel has %d registers a thread",
+                       a.numRegs);
+            checked = true;
+        }
     }
-    const int G = p.kv.n_heads / p.kv.n_kv;
-    // at most this many items; fewer than the SMs: each item's keys are split
-    const int64_t items = ((int64_t)p.rows.n_rows * G / PF_M + p.rows.n_seqs) * p.kv.n_kv;
-    const int splits = items < PF_MAX_PARTS ? (int)(PF_MAX_PARTS / items) : 1;
-    BREW_CHECK(items * splits <= 0x7fffffff, BREW_ERR_INVALID_ARG, "attention of %d rows", p.rows.n_rows);
     KvAttendParams q = p;
     q.code_base = 0x64006400u;
-    kv_prefill_kernel<R><<<(unsigned)(items * splits), PF_THREADS, smem, s>>>(q, splits);
+    kv_prefill_kernel<R><<<std::min(PF_MAX_CTAS, num_sms()), PF_THREADS, smem, s>>>(q);
     BREW_CUDA(cudaGetLastError());
     count_launch();
     return BREW_OK;
@@ -600,7 +1025,7 @@ int prefill_r(const KvAttendParams& p, cudaStream_t s) {
 bool kv_prefill_supported(int hd) { return hd == 64 || hd == 128; }
 
 int64_t kv_prefill_workspace(int hd) {
-    return kv_prefill_supported(hd) ? KV_COUNTER_BYTES + (int64_t)PF_MAX_PARTS * PF_M * (hd + 4) * 4 : 0;
+    return kv_prefill_supported(hd) ? KV_COUNTER_BYTES + (int64_t)2 * PF_MAX_CTAS * PF_M * (hd + 4) * 4 : 0;
 }
 
 int kv_prefill_launch(int hd, const KvAttendParams& p, cudaStream_t s) {
