@@ -44,7 +44,7 @@ constexpr int PF_GROUPS = PF_KT / KV_GROUP;
 constexpr int PF_RAW = 4;              // packed tiles in flight
 constexpr int PF_MAX_CTAS = 148;
 constexpr int PF_RUN = 4;              // tiles of a run, at least
-constexpr int PF_ITEM = 4;             // what an item costs beside its tiles, in tiles
+constexpr int PF_ITEM = 6;             // what an item costs beside its tiles, in tiles
 constexpr float PF_PLOG2 = 9.0f;       // p is carried times 2^9 (2^13 in tiles whose values are taken 2^-4)
 constexpr int PF_QS = 36, PF_OS = 20;  // floats from row to row where q and the output are turned: no bank twice
 
@@ -86,11 +86,11 @@ struct PfItem {
 
 struct PfRest {
     uint64_t raw_full[PF_RAW], raw_empty[PF_RAW], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_empty[2];
-    uint64_t p_full[2], p_empty[2], meta_full[4], ml_full[2], ml_empty[2], m_full[2][4], item_full[4], item_empty[4], part_full, last_full, q_full, q_empty[4], o_full[2], o_empty[2];
+    uint64_t p_full[2], p_empty[2], meta_full[4], ml_full[2], ml_empty[2], m_full[2][4], item_full[8], item_empty[8], part_full, last_full, q_full, q_empty[4], o_full[2], o_empty[2];
     uint64_t poison[4];         // of tile i & 3: its V rows with a NaN scale, a bit each
     int64_t all;                // the call's tiles and items' costs
     int ctas, len;              // CTAs that have some; this one's part
-    PfItem item[4];             // of item j & 3
+    PfItem item[8];             // of item j & 7
     uint32_t tmem;
     int last;
     float unscale[4];           // of tile i & 3: 16 where its values are taken times 2^-4
@@ -224,13 +224,13 @@ __device__ __forceinline__ bool pf_next(const KvAttendParams& p, int G, int len,
 
 // Item j of the run (n = 0: behind the last), and giving its slot back.
 __device__ __forceinline__ bool pf_item(PfRest& sh, int j, PfItem& x, unsigned int* err) {
-    if (!pf_wait_warp(&sh.item_full[j & 3], j >> 2 & 1, err)) return false;
-    x = sh.item[j & 3];
+    if (!pf_wait_warp(&sh.item_full[j & 7], j >> 3 & 1, err)) return false;
+    x = sh.item[j & 7];
     return x.n > 0;
 }
 __device__ __forceinline__ void pf_item_done(PfRest& sh, int j, int lane) {
     __syncwarp();
-    if (lane == 0) mbar_arrive(&sh.item_empty[j & 3]);
+    if (lane == 0) mbar_arrive(&sh.item_empty[j & 7]);
 }
 
 // The item's q rows to tensor memory: two fp16 parts times a power of two,
@@ -241,6 +241,17 @@ template <int R>
 __device__ __forceinline__ void pf_q_at(const KvAttendParams& p, const PfItem& x, int G, int r, int64_t& at) {
     const int pi = x.pr0 + min(r, x.npairs - 1), qr = pi / G;   // missing pairs repeat the last one
     at = (int64_t)(x.e.row0 + qr) * p.ldq + (int64_t)(x.hk * G + pi - qr * G) * (32 * R);
+}
+// To L2, before it is wanted.
+template <int R>
+__device__ __forceinline__ void pf_q_ahead(const KvAttendParams& p, const PfItem& x, int G, int lane) {
+#pragma unroll 1
+    for (int r = lane; r < x.npairs; r += 32) {
+        int64_t at;
+        pf_q_at<R>(p, x, G, r, at);
+#pragma unroll
+        for (int d = 0; d < 32 * R; d += 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.q + at + d));
+    }
 }
 __device__ __forceinline__ void pf_q_load(const KvAttendParams& p, int64_t row_at, int d, int lane, float4 (&v)[8]) {
 #pragma unroll
@@ -334,16 +345,32 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
         // ---- the run: the tiles of all items end to end (entries, kv heads, pairs, keys), before each item's what it
         // costs besides, cut into equal parts
         auto entry_tiles = [&](int b) -> int64_t {   // of one kv head; 0: the other kernel's (which records bad entries)
+            KvEntry e = {};
+            if (b < p.rows.n_seqs) e = kv_check_entry(kv, p.rows, b);
+            const int mts = (int64_t)e.rows * G >= p.pairs_min ? (e.rows * G + PF_M - 1) / PF_M : 0;
+            auto cost = [&](const KvEntry& y, int mt) {
+                int hi, kmin, kmax;
+                pf_range(p, y, G, mt, hi, kmin, kmax);
+                return PF_ITEM + kmax / PF_KT + 1 - kmin / PF_KT;
+            };
             int64_t t = 0;
-            if (b < p.rows.n_seqs) {
-                const KvEntry e = kv_check_entry(kv, p.rows, b);
-                if ((int64_t)e.rows * G >= p.pairs_min)
+            if (__reduce_max_sync(0xffffffffu, mts) <= 4) {
 #pragma unroll 1
-                    for (int mt = 0; mt * PF_M < e.rows * G; ++mt) {
-                        int hi, kmin, kmax;
-                        pf_range(p, e, G, mt, hi, kmin, kmax);
-                        t += PF_ITEM + kmax / PF_KT + 1 - kmin / PF_KT;
-                    }
+                for (int mt = 0; mt < mts; ++mt) t += cost(e, mt);
+                return t;
+            }
+#pragma unroll 1
+            for (uint32_t some = __ballot_sync(0xffffffffu, mts > 0); some; some &= some - 1) {   // long ones: a lane an item
+                const int at = __ffs(some) - 1, its = __shfl_sync(0xffffffffu, mts, at);
+                KvEntry y = {};
+                y.pos0 = __shfl_sync(0xffffffffu, e.pos0, at);
+                y.rows = __shfl_sync(0xffffffffu, e.rows, at);
+                int64_t u = 0;
+#pragma unroll 1
+                for (int mt = lane; mt < its; mt += 32) u += cost(y, mt);
+#pragma unroll
+                for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+                if (lane == at) t = u;
             }
             return t;
         };
@@ -429,11 +456,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
             mbar_init(&sh.k_full[i], 4);
             mbar_init(&sh.k_empty[i], 1);
             mbar_init(&sh.v_full[i], 4);
-            mbar_init(&sh.v_empty[i], 1);
+            mbar_init(&sh.v_empty[i], 2);
             mbar_init(&sh.s_full[i], 1);
             mbar_init(&sh.s_empty[i], 4);
             mbar_init(&sh.p_full[i], 4);
-            mbar_init(&sh.p_empty[i], 1);
+            mbar_init(&sh.p_empty[i], 2);
             mbar_init(&sh.o_full[i], 1);
             mbar_init(&sh.o_empty[i], 4);
             mbar_init(&sh.ml_full[i], 8);
@@ -444,11 +471,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
         mbar_init(&sh.part_full, 8);
         mbar_init(&sh.last_full, 1);
         mbar_init(&sh.q_full, 4);
+        for (int i = 0; i < 8; ++i) {
+            mbar_init(&sh.item_full[i], 1);
+            mbar_init(&sh.item_empty[i], PF_ITEM_USERS);
+        }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&sh.q_empty[i], 1);
             mbar_init(&sh.meta_full[i], 4);
-            mbar_init(&sh.item_full[i], 1);
-            mbar_init(&sh.item_empty[i], PF_ITEM_USERS);
         }
         fence_mbar_init();
     } else if (warp == 1) {
@@ -466,13 +495,21 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
     if (warp < PF_W_SOFT) {
         regs_dec<PF_REGS_ISSUE>();
         if (warp == 0 && len > 0) {
-            // ---------------- copies: a group of 16 positions a lane ----------------
+            // ---------------- the run's items, and their copies: a group of 16 positions a lane ----------------
             const int per = 1 << (kv.page_shift - 4);
-            PfItem x;
+            PfItem x = sh.item[0];
             int i = 0;
             bool ok = true;
 #pragma unroll 1
-            for (int j = 0; ok && pf_item(sh, j, x, kv.err); ++j) {
+            for (int j = 0; ok; ++j) {
+                if (j > 0) {
+                    if (!pf_next(p, G, len, x)) x.n = 0;
+                    if (!pf_wait_warp(&sh.item_empty[j & 7], (j >> 3 & 1) ^ 1, kv.err)) break;
+                    if (lane == 0) sh.item[j & 7] = x;
+                }
+                if (lane == 0) mbar_arrive(&sh.item_full[j & 7]);
+                if (x.n == 0) break;
+                if (j > 0) pf_q_ahead<R>(p, x, G, lane);
                 const int32_t* pages = kv.table + (int64_t)x.e.seq * kv.max_pages;
                 auto page_of = [&](int t) {
                     const int pos = (x.ta + t) * PF_KT + 16 * lane;
@@ -495,7 +532,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
                     }
                     id = page_of(t + 1);
                 }
-                pf_item_done(sh, j, lane);
             }
         } else if (warp == 1 && len > 0) {
             // ---------------- MMA issue: S = q k ----------------
@@ -531,10 +567,14 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
                 }
                 pf_item_done(sh, j, lane);
             }
-        } else if (warp == 2 && len > 0) {
-            // ---------------- MMA issue: O = p v, half of the dims at a time: one is read while the other is made ----------------
+        } else if (warp >= 2 && len > 0) {
+            // ---------------- MMA issue: O = p v, a warp for each half of the dims ----------------
             constexpr uint32_t idesc = umma_idesc_f16(PF_M, HD / 2);
-            const uint64_t vdesc = umma_desc_k(smem_u32(smem + S::V), S::V_PIECE, S::V_GROUP);
+            const int h = warp - 2;
+            if (h == 1)   // the first item's q rows to L2
+                pf_q_ahead<R>(p, sh.item[0], G, lane);
+            const uint32_t to = tmem + PF_T_O + h * (HD / 2);
+            const uint64_t vdesc = umma_desc_k(smem_u32(smem + S::V), S::V_PIECE, S::V_GROUP) + h * (HD / 16 * S::V_GROUP / 16);
             PfItem x;
             int j = 0, tiles = 0;
             bool ok = true;
@@ -546,52 +586,24 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
                     pf_item_done(sh, j++, lane);
                 }
                 const int b = i & 1;
-                ok = pf_wait_warp(&sh.p_full[b], i >> 1 & 1, kv.err) && pf_wait_warp(&sh.v_full[b], i >> 1 & 1, kv.err);
-#pragma unroll 1
-                for (int h = 0; h < 2 && ok; ++h) {
-                    ok = pf_wait_warp(&sh.o_empty[h], (i & 1) ^ 1, kv.err);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint64_t hi = vdesc + b * (2 * S::V_PART / 16) + h * (HD / 16 * S::V_GROUP / 16);
-                        const uint32_t tp = tmem + PF_T_P + b * PF_KT, to = tmem + PF_T_O + h * (HD / 2);
+                ok = pf_wait_warp(&sh.v_full[b], i >> 1 & 1, kv.err) && pf_wait_warp(&sh.o_empty[h], (i & 1) ^ 1, kv.err) &&
+                     pf_wait_warp(&sh.p_full[b], i >> 1 & 1, kv.err);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t hi = vdesc + b * (2 * S::V_PART / 16);
+                    const uint32_t tp = tmem + PF_T_P + b * PF_KT;
 #pragma unroll
-                        for (int pass = 0; pass < 3; ++pass)
+                    for (int pass = 0; pass < 3; ++pass)
 #pragma unroll
-                            for (int s = 0; s < PF_KT / 16; ++s)
-                                umma_f16_ts(to, tp + (pass == 0 ? PF_KT / 2 : 0) + 8 * s,
-                                            hi + ((pass == 1 ? S::V_PART : 0) + s * 2 * S::V_PIECE) / 16, idesc, pass + s > 0);
-                        umma_commit(&sh.o_full[h]);
-                        if (h == 1) {
-                            umma_commit(&sh.v_empty[b]);
-                            umma_commit(&sh.p_empty[b]);
-                        }
-                    }
-                    __syncwarp();
+                        for (int s = 0; s < PF_KT / 16; ++s)
+                            umma_f16_ts(to, tp + (pass == 0 ? PF_KT / 2 : 0) + 8 * s,
+                                        hi + ((pass == 1 ? S::V_PART : 0) + s * 2 * S::V_PIECE) / 16, idesc, pass + s > 0);
+                    umma_commit(&sh.o_full[h]);
+                    umma_commit(&sh.v_empty[b]);
+                    umma_commit(&sh.p_empty[b]);
                 }
-            }
-        } else if (warp == 3 && len > 0) {
-            // ---------------- the run's items, and their q rows to L2 ----------------
-            PfItem x = sh.item[0];
-            bool more = true;
-#pragma unroll 1
-            for (int j = 0; more; ++j) {
-                if (j > 0) {
-                    more = pf_next(p, G, len, x);
-                    if (!pf_wait_warp(&sh.item_empty[j & 3], (j >> 2 & 1) ^ 1, kv.err)) break;
-                    if (!more) x.n = 0;
-                    if (lane == 0) sh.item[j & 3] = x;
-                    __syncwarp();
-                }
-                if (lane == 0) mbar_arrive(&sh.item_full[j & 3]);
-                if (j == 0 || !more) continue;
-#pragma unroll 1
-                for (int r = lane; r < x.npairs; r += 32) {
-                    int64_t at;
-                    pf_q_at<R>(p, x, G, r, at);
-#pragma unroll
-                    for (int d = 0; d < HD; d += 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.q + at + d));
-                }
+                __syncwarp();
             }
         }
         __syncwarp();
@@ -666,36 +678,39 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
                     tc_fence_after();
                     uint64_t sum = f2_packf(0.0f, 0.0f);
 #pragma unroll 1
-                    for (int h = 0; h < 4; ++h) {
-                        float v[16];
-                        tmem_ld16(ts + 16 * h, v);
+                    for (int h = 0; h < 2; ++h) {
+                        float v[32];
+                        tmem_ld32(ts + 32 * h, v);
                         tmem_ld_wait();
-                        if (h == 3) {
+                        if (h == 1) {
                             tc_fence_before();
                             __syncwarp();
                             if (lane == 0) mbar_arrive(&sh.s_empty[b]);
                         }
                         if (!full) {
-                            const uint32_t s16 = (uint32_t)(see >> 16 * h);
+                            const uint32_t s32 = (uint32_t)(see >> 32 * h);
 #pragma unroll
-                            for (int c = 0; c < 16; ++c)
-                                if (!(s16 >> c & 1)) v[c] = -INFINITY;
+                            for (int c = 0; c < 32; ++c)
+                                if (!(s32 >> c & 1)) v[c] = -INFINITY;
                         }
-                        uint32_t hi[8], lo[8];
 #pragma unroll
-                        for (int y = 0; y < 16; y += 2) {
-                            const float2 a = f2_float2(f2_fma(f2_packf(v[y], v[y + 1]), f2, mref2));
-                            const float p0 = ex2(a.x), p1 = ex2(a.y);
-                            const uint64_t pp = f2_packf(p0, p1);
-                            sum = f2_add(sum, pp);
-                            const __half2 ph = __floats2half2_rn(p0, p1);
-                            const float2 pf = __half22float2(ph);
-                            hi[y / 2] = *reinterpret_cast<const uint32_t*>(&ph);
-                            const float2 rest = f2_float2(f2_fma(f2_packf(pf.x, pf.y), minus, pp));
-                            lo[y / 2] = pack_half2(rest.x, rest.y);
+                        for (int c = 0; c < 32; c += 16) {
+                            uint32_t hi[8], lo[8];
+#pragma unroll
+                            for (int y = 0; y < 16; y += 2) {
+                                const float2 a = f2_float2(f2_fma(f2_packf(v[c + y], v[c + y + 1]), f2, mref2));
+                                const float p0 = ex2(a.x), p1 = ex2(a.y);
+                                const uint64_t pp = f2_packf(p0, p1);
+                                sum = f2_add(sum, pp);
+                                const __half2 ph = __floats2half2_rn(p0, p1);
+                                const float2 pf = __half22float2(ph);
+                                hi[y / 2] = *reinterpret_cast<const uint32_t*>(&ph);
+                                const float2 rest = f2_float2(f2_fma(f2_packf(pf.x, pf.y), minus, pp));
+                                lo[y / 2] = pack_half2(rest.x, rest.y);
+                            }
+                            tmem_st8(tp + 16 * h + c / 2, hi);
+                            tmem_st8(tp + PF_KT / 2 + 16 * h + c / 2, lo);
                         }
-                        tmem_st8(tp + 8 * h, hi);
-                        tmem_st8(tp + PF_KT / 2 + 8 * h, lo);
                     }
                     const float2 sf = f2_float2(sum);
                     l = fmaf(sf.x + sf.y, up == 1.0f ? 1.0f : 0.0625f, l);
@@ -823,13 +838,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
                     ++cuts;
                     if (sh.last) {
                         float M = -INFINITY, L = 0.0f;
-#pragma unroll 1
-                        for (int k = 0; k < parts; ++k)
-                            M = fmaxf(M, __ldcg(reinterpret_cast<const float2*>(part(k) + PF_M * HD) + r).x);
-#pragma unroll 1
+#pragma unroll 4
                         for (int k = 0; k < parts; ++k) {
                             const float2 y = __ldcg(reinterpret_cast<const float2*>(part(k) + PF_M * HD) + r);
-                            L += y.y * (y.x == -INFINITY ? 0.0f : ex2(y.x - M));
+                            const float n = fmaxf(M, y.x);
+                            L = L * (M == n ? 1.0f : ex2(M - n)) + y.y * (y.x == -INFINITY ? 0.0f : ex2(y.x - n));
+                            M = n;
                         }
                         const float inv = 1.0f / L;
 #pragma unroll 1
@@ -837,19 +851,26 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
                             float v[16];
 #pragma unroll
                             for (int k = 0; k < 16; ++k) v[k] = 0.0f;
-#pragma unroll 2
+                            const float4* at = reinterpret_cast<const float4*>(part(0)) + (w8 * (NC / 4) + c / 4) * 32 + lane;
+                            const float2* ml = reinterpret_cast<const float2*>(part(0) + PF_M * HD) + r;
+                            // (the first part is the second of its CTA's, the others are the first of theirs)
+                            constexpr int64_t STEP = PF_M * (HD + 4) / 4;
+#pragma unroll 4
                             for (int k = 0; k < parts; ++k) {
-                                const float my = __ldcg(reinterpret_cast<const float2*>(part(k) + PF_M * HD) + r).x;
+                                const float my = __ldcg(ml).x;
+                                float4 z[4];
+#pragma unroll
+                                for (int y = 0; y < 4; ++y) z[y] = __ldcg(at + 32 * y);
                                 const float a = my == -INFINITY ? 0.0f : ex2(my - M) * inv;
 #pragma unroll
                                 for (int y = 0; y < 4; ++y) {
-                                    const float4 z =
-                                        __ldcg(reinterpret_cast<const float4*>(part(k)) + (w8 * (NC / 4) + c / 4 + y) * 32 + lane);
-                                    v[4 * y] += a * z.x;
-                                    v[4 * y + 1] += a * z.y;
-                                    v[4 * y + 2] += a * z.z;
-                                    v[4 * y + 3] += a * z.w;
+                                    v[4 * y] += a * z[y].x;
+                                    v[4 * y + 1] += a * z[y].y;
+                                    v[4 * y + 2] += a * z[y].z;
+                                    v[4 * y + 3] += a * z[y].w;
                                 }
+                                at += k == 0 ? STEP : 2 * STEP;
+                                ml += k == 0 ? 2 * STEP : 4 * STEP;
                             }
                             write(c, v);
                         }
