@@ -525,3 +525,140 @@ def test_attend_is_deterministic(device):
     first = f.attend(q, e)
     for _ in range(5):
         assert torch.equal(first, f.attend(q, e))
+
+
+# ---- prompts: many rows of a sequence ------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd", [(2, 2, 64), (3, 1, 128), (10, 2, 128), (7, 1, 64), (96, 1, 64), (128, 1, 128)])
+@pytest.mark.parametrize("window", [0, 1, 63, 64, 65, 200, 5000])
+def test_prompt_windows_and_groups(device, heads, kv_heads, hd, window):
+    """Heads of a row in two tiles of pairs, rows of a tile that see different tiles of keys, pages of every size."""
+    page = {0: 16, 1: 32, 63: 64, 64: 128}.get(window, 16)
+    f = Filled(heads, kv_heads, hd, [391, 64, 129], page, seed=heads + window)
+    entries = [(0, 391 - 150, 150), (1, 0, 64), (2, 128, 1), (2, 0, 129), (0, 5, 66)]
+    f.check(f.q(sum(e[2] for e in entries)), entries, window)
+
+
+def test_prompt_over_every_cta(device):
+    """128 pairs whose keys all of the device's CTAs share; two of them beside short ones."""
+    f = Filled(2, 1, 128, [38001, 90, 300], 64, seed=41)
+    f.check(f.q(64), [(0, 38001 - 64, 64)])
+    f.check(f.q(64 + 90 + 70), [(1, 0, 90), (0, 20000, 64), (2, 230, 70)])
+
+
+def test_prompts_among_single_tokens(device):
+    """More than 32 and more than 256 entries, one kernel's and the other's in turn, empty ones between."""
+    lens = [1 + (i * 53) % 170 for i in range(300)]
+    f = Filled(4, 2, 64, lens, 16, seed=42)
+    entries = [(i, n - 1, 1) if i % 3 else (i, 0, n) if i % 2 else (i, n // 2, n - n // 2) for i, n in enumerate(lens)]
+    entries[7] = (7, 3, 0)
+    f.check(f.q(sum(e[2] for e in entries)), entries)
+    f.check(f.q(sum(e[2] for e in entries)), entries, window=40)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kgain,vgain,qgain", [(4e4, 1.0, 1e-4), (1e-7, 4e5, 1e6), (1.0, 1e-7, 1.0), (4e5, 4e5, 1e-6)])
+def test_prompt_magnitudes(device, hd, kgain, vgain, qgain):
+    """Scales at both ends of fp16, tiles of large ones between tiles of small ones."""
+    f = Filled(6, 2, hd, [330], 32, seed=43)
+    k = torch.randn(330, 2, hd, generator=f.g, device=DEV)
+    v = torch.randn(330, 2, hd, generator=f.g, device=DEV)
+    k[100:150] *= kgain
+    v[60:200] *= vgain
+    f.kv.append(0, 0, 0, 0, k.data_ptr(), v.data_ptr(), 2 * hd, make_rows([(0, 0, 330)]))
+    f.k, f.v = [stored(k)], [stored(v)]
+    f.check(f.q(130, qgain), [(0, 200, 130)])
+    f.check(f.q(70, qgain), [(0, 100, 70)])
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd", [(4, 2, 64), (6, 1, 128)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_prompt_rows_before_a_nan(device, heads, kv_heads, hd, window):
+    """A value or key of a chunk that is NaN reaches the rows that see it and no others."""
+    for what in "kv":
+        f = Filled(heads, kv_heads, hd, [300], 64, seed=44)
+        x = torch.randn(1, kv_heads, hd, generator=f.g, device=DEV)
+        y = x.clone()
+        (y if what == "v" else x)[:, 0, 32:64] = float("nan")
+        f.kv.append(0, 0, 0, 0, x.data_ptr(), y.data_ptr(), kv_heads * hd, make_rows([(0, 210, 1)]))
+        q = f.q(180)
+        got = f.attend(q, [(0, 120, 180)], window)
+        f.kv.check()
+        want, tol = f.expected(q, [(0, 120, 180)], window)   # (with another key 210: right for the rows without it)
+        row = torch.arange(120, 300, device=DEV)
+        sees = (row >= 210) & ((row < 210 + window) if window else row >= 0)
+        assert bool(((got[~sees].double() - want[~sees]).abs() <= tol[~sees]).all())
+        g = heads // kv_heads
+        part = slice(32, 64) if what == "v" else slice(None)
+        assert torch.isnan(got[sees][:, :g, part]).all()
+
+
+def test_prompt_nan_row_stays_alone(device):
+    f = Filled(4, 2, 128, [200], 16, seed=45)
+    q = f.q(150)
+    q[70, 1, 5] = float("nan")
+    got = f.attend(q, [(0, 50, 150)])
+    f.kv.check()
+    want, tol = f.expected(torch.nan_to_num(q), [(0, 50, 150)])
+    bad = torch.zeros(150, 4, dtype=torch.bool, device=DEV)
+    bad[70, 1] = True
+    assert torch.isnan(got[bad]).all()
+    assert bool(((got.double() - want).abs() <= tol)[~bad].all())
+
+
+def test_prompt_strides_and_rows_behind(device):
+    f = Filled(6, 2, 64, [150, 80], 32, seed=46)
+    ld, n = 6 * 64 + 4, 100 + 80 + 9
+    q = torch.randn(n, ld, generator=f.g, device=DEV)
+    out = torch.full((n, ld + 8), 7.0, device=DEV)
+    entries = [(0, 50, 100), (1, 0, 80)]
+    f.kv.attend(0, out.data_ptr(), ld + 8, q.data_ptr(), ld, make_rows(entries, n), 0, f.ws.data_ptr(), -0.2)
+    f.kv.check()
+    want, tol = f.expected(q[:180, :384].reshape(180, 6, 64), entries, 0, -0.2)
+    assert bool(((out[:180, :384].reshape(180, 6, 64).double() - want).abs() <= tol.abs()).all())
+    assert bool((out[180:] == 7).all()) and bool((out[:, 384:] == 7).all())
+
+
+def test_prompt_graphs_beside_each_other(device):
+    """Two captured calls, a workspace each, replayed at once on their own streams; the same bits each time."""
+    f = Filled(16, 4, 128, [900, 3000, 70], 64, seed=47)
+    rows = [make_rows([(0, 300, 600), (2, 69, 1)]), make_rows([(1, 2800, 200), (2, 0, 70), (0, 899, 1)])]
+    qs = [f.q(601), f.q(271)]
+    outs = [torch.empty_like(q) for q in qs]
+    spaces = [torch.zeros(f.kv.workspace_bytes(), dtype=torch.uint8, device=DEV) for _ in qs]
+    torch.cuda.synchronize()
+    graphs, streams = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for r, q, o, w in zip(rows, qs, outs, spaces):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            f.kv.attend(0, o.data_ptr(), 2048, q.data_ptr(), 2048, r, 0, w.data_ptr(),
+                        stream=torch.cuda.current_stream().cuda_stream)
+        graphs.append(gr)
+    first = None
+    for _ in range(4):
+        for o in outs:
+            o.fill_(math.nan)
+        torch.cuda.synchronize()
+        for gr, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                gr.replay()
+        torch.cuda.synchronize()
+        f.kv.check()
+        first = first or [o.clone() for o in outs]
+        assert all(torch.equal(a, b) for a, b in zip(first, outs))
+    for q, o, e in zip(qs, first, ([(0, 300, 600), (2, 69, 1)], [(1, 2800, 200), (2, 0, 70), (0, 899, 1)])):
+        want, tol = f.expected(q, e)
+        assert bool(((o.double() - want).abs() <= tol).all())
+
+
+def test_prompt_bad_entries_between_good_ones(device):
+    f = Filled(8, 2, 128, [200, 150], 16, seed=48)
+    q = f.q(100 + 80 + 90)
+    got = f.attend(q, [(0, 100, 100), (1, 100, 80), (1, 60, 90)])   # the second: behind what is reserved
+    with pytest.raises(N.IllegalStateException):
+        f.kv.check()
+    for part, e in ((slice(0, 100), (0, 100, 100)), (slice(180, 270), (1, 60, 90))):
+        want, tol = f.expected(q[part].contiguous(), [e])
+        assert bool(((got[part].double() - want).abs() <= tol).all())
+    assert torch.isnan(got[100:180]).all()
