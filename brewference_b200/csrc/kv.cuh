@@ -84,6 +84,7 @@ struct KvAttendParams {
     float scale;
     void* workspace;
     uint32_t code_base;        // set by the launch
+    int prompts;               // the prompt kernel follows
     int64_t pairs_min;         // entries of fewer (row, head) pairs a kv head are the single-token kernel's, the others
                                // the prompt kernel's
 };

@@ -39,8 +39,14 @@ constexpr int AT_MAX_CTAS = 4 * 148;
 // mma truncates as it accumulates: after this many tiles its sums are added,
 // rounded, to others (128 x 8192 positions: error 3.0e-6 without).
 constexpr int AT_FLUSH = 8;
-// From this many (row, head) pairs of an entry and kv head on, the prompt kernel takes it.
-constexpr int64_t AT_PROMPT_PAIRS = 64;
+// From this many (row, head) pairs of an entry and kv head on, the prompt
+// kernel takes it: its tiles of 128 pairs cost the same however few there are,
+// but no more than this kernel's 8 tiles of 8.  32 sequences of 1000 positions
+// with 64 pairs each, 16/8 heads of 128: 77 us there, 121 here; with 16 pairs
+// 71 and 43.  In a call of few rows, where neither fills the device, this
+// kernel starts faster: one sequence of 300 positions with 256 pairs, 30 us
+// there, 23 here; of 4096 positions with 256 pairs 41 and 57, with 64 39 and 30.
+constexpr int64_t AT_PROMPT_PAIRS = 64, AT_PROMPT_PAIRS_FEW = 256, AT_MANY_PAIRS = 2048;
 constexpr float AT_LAZY = 2.0f;                   // log2 of how far p may exceed 1
 
 template <int R>
@@ -147,6 +153,7 @@ __global__ void __launch_bounds__(AtShape<R>::THREADS, AtShape<R>::CTAS_PER_SM)
     constexpr int HD = S::HD;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, i = lane & 3;
+    if (p.prompts) pdl_launch_dependents();   // it shares nothing with this kernel's work: other entries, another workspace
     uint8_t* ring = smem + warp * S::RING;
     float* mine = reinterpret_cast<float*>(smem + S::WARPS * S::RING + warp * S::SUMS);
     uint4* qs = reinterpret_cast<uint4*>(smem + S::Q);                 // [block][hi, lo][lane]
@@ -686,15 +693,18 @@ int attend_r(const KvAttendParams& p, cudaStream_t s) {
 
 }  // namespace
 
-int64_t kv_attend_workspace(int head_size) {
-    return std::max(KV_COUNTER_BYTES + (int64_t)AT_MAX_CTAS * 2 * at_part_floats(head_size) * 4,
-                    kv_prefill_workspace(head_size));
+// The single-token kernel's part of the workspace; the prompt kernel's lies behind it.
+static int64_t at_workspace(int head_size) {
+    return KV_COUNTER_BYTES + ((int64_t)AT_MAX_CTAS * 2 * at_part_floats(head_size) * 4 + 255) / 256 * 256;
 }
+int64_t kv_attend_workspace(int head_size) { return at_workspace(head_size) + kv_prefill_workspace(head_size); }
 
 int kv_attend_launch(int hd, const KvAttendParams& p0, cudaStream_t s) {
     KvAttendParams p = p0;
     const int64_t most = (int64_t)p.rows.max_rows * (p.kv.n_heads / p.kv.n_kv);
-    p.pairs_min = kv_prefill_supported(hd) ? AT_PROMPT_PAIRS : INT64_MAX;
+    p.pairs_min = !kv_prefill_supported(hd) ? INT64_MAX
+                  : (int64_t)p.rows.n_rows * p.kv.n_heads >= AT_MANY_PAIRS ? AT_PROMPT_PAIRS : AT_PROMPT_PAIRS_FEW;
+    p.prompts = most >= p.pairs_min;
     int rc;
     switch (hd / 32) {
         case 1: rc = attend_r<1>(p, s); break;
@@ -703,7 +713,9 @@ int kv_attend_launch(int hd, const KvAttendParams& p0, cudaStream_t s) {
         case 4: rc = attend_r<4>(p, s); break;
         default: rc = attend_r<8>(p, s); break;
     }
-    return rc || most < p.pairs_min ? rc : kv_prefill_launch(hd, p, s);
+    if (rc || !p.prompts) return rc;
+    p.workspace = static_cast<uint8_t*>(p.workspace) + at_workspace(hd);
+    return kv_prefill_launch(hd, p, s);
 }
 
 }  // namespace brew

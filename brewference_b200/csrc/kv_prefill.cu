@@ -14,20 +14,32 @@
 // starts at 0 and is added in fp32 registers with the softmax's correction,
 // because accumulation in tensor memory truncates.
 //
-// The tiles of all items, end to end, are cut into one equal run a CTA; items
-// that a cut divides leave parts (O, maximum, sum) in the workspace, which the
-// last of their CTAs joins.
+// The tiles of all items, end to end, are cut into one equal run a CTA, an
+// item's beginning and end (q, the output, a pipeline that empties) weighing 6
+// tiles (2: 156 us, 4: 126, 6: 117, 9: 118 for ragged prompts of up to 700
+// rows).  Items that a cut divides leave parts (O, maximum, sum) in the
+// workspace, which the last of their CTAs joins.
 //
-// Warps: one copies the tiles' packed groups (bulk copies), one issues the
-// MMAs, two warpgroups take turns at the softmax of a tile (a thread is a row;
-// the running maximum passes between them), two add up O (a thread is half a
-// row), two take turns at unpacking a tile's K and V and at bringing an item's
-// q.  K, V, S, P and the packed tiles are buffered twice or more and the rings
-// go on from item to item; QK of the next tile is issued before PV of the
-// present one, so the tensor cores work while the softmax does.
+// 28 warps, the registers divided among them:
+//   0        walks the run's items (a ring of descriptions in shared memory that
+//            the others read) and copies their packed tiles (bulk copies)
+//   1        issues q k, 24 MMAs of 64 columns a tile
+//   2, 3     issue p v, a warp for each half of the dims: one half of O is read
+//            while the other is made
+//   4 .. 11  softmax: two warpgroups, every other tile; a thread is a row.  The
+//            running maximum passes from one tile to the next in shared memory.
+//   12 .. 19 add up O: a thread is half a row
+//   20 .. 27 unpack: a warpgroup for K, which brings q too, one for V
+// K, V, S, P and the packed tiles have two buffers or more, and the rings go on
+// from item to item.
 //
-// Bound: the tensor cores, 1730 cycles a tile of 64 keys x 128 pairs x 128
-// dims (24 products of 64 columns at 37, 12 of 128 at 70).
+// Measured: a tile of 64 keys takes 1.4 us a CTA, where its 48 MMAs of 37
+// cycles take 1.0 (a chunk of 512 rows at 4096 positions, 16/8 heads of 128:
+// 64 us, of which 12 until the first product and 8 from the last to the joined
+// output).  What bounds it is the other warps' work beside them: 7800 warp
+// instructions a tile at 45% of the issue slots, in loops that have to stay in
+// the instruction cache together (the waits as a dozen instructions each, not
+// forty, took 15% off).
 #include <algorithm>
 
 #include "brew_internal.cuh"
@@ -1007,6 +1019,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
     }
     tc_fence_before();
     __syncthreads();
+    pdl_wait();   // the single-token kernel: what comes after this one on the stream comes after both
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
@@ -1035,8 +1048,18 @@ int prefill_r(const KvAttendParams& p, cudaStream_t s) {
     }
     KvAttendParams q = p;
     q.code_base = 0x64006400u;
-    kv_prefill_kernel<R><<<std::min(PF_MAX_CTAS, num_sms()), PF_THREADS, smem, s>>>(q);
-    BREW_CUDA(cudaGetLastError());
+    // starts beside the single-token kernel of the call, which has nothing to do where all entries are prompts
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(std::min(PF_MAX_CTAS, num_sms()));
+    cfg.blockDim = dim3(PF_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    BREW_CUDA(cudaLaunchKernelEx(&cfg, kv_prefill_kernel<R>, q));
     count_launch();
     return BREW_OK;
 }

@@ -662,3 +662,18 @@ def test_prompt_bad_entries_between_good_ones(device):
         want, tol = f.expected(q[part].contiguous(), [e])
         assert bool(((got[part].double() - want).abs() <= tol).all())
     assert torch.isnan(got[100:180]).all()
+
+
+def test_prompt_of_few_rows_over_every_cta(device):
+    """Two tiles of pairs whose keys all of the device's CTAs share, many parts to join."""
+    f = Filled(2, 1, 64, [50003, 130], 32, seed=49)
+    f.check(f.q(128), [(0, 50003 - 128, 128)])
+    f.check(f.q(128 + 130), [(1, 0, 130), (0, 31000, 128)])
+
+
+@pytest.mark.parametrize("rows", [15, 16, 17, 63, 64, 65])
+def test_rows_on_both_sides_of_the_kernels_limits(device, rows):
+    """4 heads a kv head: 64 pairs among many rows, 256 among few."""
+    f = Filled(8, 2, 64, [300, 300, 300, 300], 16, seed=50)
+    f.check(f.q(rows), [(0, 300 - rows, rows)])
+    f.check(f.q(rows + 16 + 300), [(1, 100, rows), (2, 0, 16), (3, 0, 300)])
