@@ -13,8 +13,13 @@
 // Top alternatives: every warp keeps the 32 largest of its logits as sorted
 // 64-bit keys (the logit's order, then the lower index), one a lane.  A logit
 // is a candidate only when it beats the warp's own `top`-th and reaches the
-// CTA's floor, which the warps make together three times a row; 32 candidates are sorted and joined with the list at a time (an exchange
-// and five steps).  In rising rows every logit is a candidate.
+// CTA's floor, which the warps make together three times a row; 32 candidates
+// are sorted and joined with the list at a time (an exchange and five steps).
+// In rising rows every logit is a candidate.
+//
+// 1777 rows of 151936: 222 us with 20 alternatives (0.74 of a copy's rate), 171
+// without (0.96).  (An insertion per candidate 508; a floor of each warp's own
+// 357; of the CTA's, from sorted lists 310, from the lanes' largest 222.)
 #include <algorithm>
 
 #include "brew_internal.cuh"
