@@ -184,14 +184,17 @@ JNIEXPORT void JNICALL Java_com_epicmonstrosity_brewference_gpu_Brew_score(JNIEn
         if (c) env->ThrowNew(c, "an array shorter than the tokens to score");
         return;
     }
-    std::vector<int32_t> t(n > 0 ? n : 1);
-    if (n > 0) env->GetIntArrayRegion(tokens, 0, n, reinterpret_cast<jint*>(t.data()));
+    jint* t = tokens ? env->GetIntArrayElements(tokens, nullptr) : nullptr;
     jfloat* lp = logprob ? env->GetFloatArrayElements(logprob, nullptr) : nullptr;
     jfloat* en = entropy ? env->GetFloatArrayElements(entropy, nullptr) : nullptr;
-    const int rc = brew_session_score(reinterpret_cast<brew_model>(m), tokens ? t.data() : nullptr, n, 0, lp, en, nullptr,
-                                      nullptr);
+    const bool all = (t || !tokens) && (lp || !logprob) && (en || !entropy);   // else an OutOfMemoryError is pending
+    const int rc = all ? brew_session_score(reinterpret_cast<brew_model>(m), reinterpret_cast<int32_t*>(t), n, 0, lp, en,
+                                            nullptr, nullptr)
+                       : BREW_ERR_CUDA;
+    if (t) env->ReleaseIntArrayElements(tokens, t, JNI_ABORT);
     if (lp) env->ReleaseFloatArrayElements(logprob, lp, rc ? JNI_ABORT : 0);
     if (en) env->ReleaseFloatArrayElements(entropy, en, rc ? JNI_ABORT : 0);
+    if (!all) return;
     if (rc) throw_for(env, rc);
 }
 

@@ -53,6 +53,15 @@ int set_pages(brew_kv_s* kv, int seq, size_t first, size_t end, int tokens, cuda
     return BREW_OK;
 }
 
+// Pages change hands once, on the host: a replayed graph would do it again.
+int not_captured(cudaStream_t s) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    BREW_CUDA(cudaStreamIsCapturing(s, &st));
+    BREW_CHECK(st == cudaStreamCaptureStatusNone, BREW_ERR_INVALID_ARG,
+               "pages cannot be reserved or released while the stream is captured");
+    return BREW_OK;
+}
+
 // ---- append -------------------------------------------------------------
 // The 4-bit code of a value next to a rounding border depends on its last
 // bit (and a position of 10^5 leaves 32 bits no digit of the angle), so
@@ -475,6 +484,8 @@ int brew_kv_reserve(brew_kv kv, int32_t seq, int32_t n_tokens, void* stream) {
     std::vector<int32_t>& have = kv->seq_pages[seq];
     const size_t need = ((size_t)n_tokens + kv->c.page_tokens - 1) >> kv->page_shift, first = have.size();
     if (need <= first) return BREW_OK;
+    int rc = not_captured(static_cast<cudaStream_t>(stream));
+    if (rc) return rc;
     BREW_CHECK(need - first <= kv->free_pages.size(), BREW_ERR_CONTEXT_FULL,
                "K/V cache: %zu pages needed, %zu free", need - first, kv->free_pages.size());
     try {
@@ -486,7 +497,9 @@ int brew_kv_reserve(brew_kv kv, int32_t seq, int32_t n_tokens, void* stream) {
         have.push_back(kv->free_pages.back());
         kv->free_pages.pop_back();
     }
-    return set_pages(kv, seq, first, need, (int)(need << kv->page_shift), static_cast<cudaStream_t>(stream));
+    rc = set_pages(kv, seq, first, need, (int)(need << kv->page_shift), static_cast<cudaStream_t>(stream));
+    for (; rc && have.size() > first; have.pop_back()) kv->free_pages.push_back(have.back());
+    return rc;
 }
 
 int brew_kv_release(brew_kv kv, int32_t seq, void* stream) {
@@ -496,8 +509,8 @@ int brew_kv_release(brew_kv kv, int32_t seq, void* stream) {
     if (ds.rc) return ds.rc;
     std::lock_guard<std::mutex> lk(kv->mu);
     std::vector<int32_t>& have = kv->seq_pages[seq];
-    int rc = set_pages(kv, seq, 0, 0, 0, static_cast<cudaStream_t>(stream));
-    if (rc) return rc;
+    int rc = not_captured(static_cast<cudaStream_t>(stream));
+    if (rc || (rc = set_pages(kv, seq, 0, 0, 0, static_cast<cudaStream_t>(stream)))) return rc;
     // free_pages was sized for every page: no allocation here
     for (size_t i = have.size(); i-- > 0;) kv->free_pages.push_back(have[i]);
     have.clear();

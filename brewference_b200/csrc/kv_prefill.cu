@@ -578,6 +578,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
                     __syncwarp();
                 }
                 pf_item_done(sh, j, lane);
+                // the last commit has arrived before the CTA ends
+                if (ok && x.off + x.cnt + PF_ITEM >= len) pf_wait_warp(&sh.q_empty[j & 3], j >> 2 & 1, kv.err);
             }
         } else if (warp >= 2 && len > 0) {
             // ---------------- MMA issue: O = p v, a warp for each half of the dims ----------------
@@ -593,7 +595,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
 #pragma unroll 1
             for (int i = 0; ok; ++i) {
                 if (i == tiles) {
-                    if (!pf_item(sh, j, x, kv.err)) break;
+                    if (!pf_item(sh, j, x, kv.err)) {   // the end: the last commit has arrived before the CTA ends
+                        if (i > 0) pf_wait_warp(&sh.p_empty[(i - 1) & 1], (i - 1) >> 1 & 1, kv.err);
+                        break;
+                    }
                     tiles += x.n;
                     pf_item_done(sh, j++, lane);
                 }

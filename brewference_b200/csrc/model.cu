@@ -1713,9 +1713,9 @@ int brew_model_set_kv_cache(brew_model m, int32_t type) {
     if ((rc = alloc_unfused(m))) return rc;
     const int B = m->max_batch;
     if (!m->kv_rows && (rc = dalloc(m, &m->kv_rows, (size_t)B + 4))) return rc;
-    std::vector<int32_t> ids(B);
+    int32_t ids[MODEL_MAX_BATCH];
     for (int b = 0; b < B; ++b) ids[b] = b;
-    BREW_CUDA(cudaMemcpy(m->kv_rows, ids.data(), B * sizeof(int32_t), cudaMemcpyHostToDevice));
+    BREW_CUDA(cudaMemcpy(m->kv_rows, ids, B * sizeof(int32_t), cudaMemcpyHostToDevice));
     if (!m->kv_ws) {
         uint8_t* ws = nullptr;
         if ((rc = dalloc(m, &ws, (size_t)kv_attend_workspace(c.head_size)))) return rc;

@@ -423,7 +423,8 @@ BREW_API int brew_selftest_wait_timeout(int64_t limit_ns, int32_t* waits_ended);
  * n_tokens - 1 (it only grows; BREW_ERR_CONTEXT_FULL past max_tokens or when
  * the pool is empty, nothing is changed then), brew_kv_release returns them
  * all.  Both take effect on the device in `stream` order; a page released on
- * one stream and taken on another needs an ordering between the two.
+ * one stream and taken on another needs an ordering between the two.  Neither
+ * can be captured into a CUDA graph (BREW_ERR_INVALID_ARG).
  *
  * The _dev calls take device pointers and enqueue on `stream` (0 = default)
  * without synchronising or allocating; they can be captured into a CUDA

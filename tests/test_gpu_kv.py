@@ -677,3 +677,25 @@ def test_rows_on_both_sides_of_the_kernels_limits(device, rows):
     f = Filled(8, 2, 64, [300, 300, 300, 300], 16, seed=50)
     f.check(f.q(rows), [(0, 300 - rows, rows)])
     f.check(f.q(rows + 16 + 300), [(1, 100, rows), (2, 0, 16), (3, 0, 300)])
+
+
+def test_pages_do_not_change_hands_in_a_captured_stream(device):
+    """A replay would hand them out again: refused, and nothing is changed."""
+    kv = KvCache(1, 2, 1, 64, 2, 64, 16)
+    kv.reserve(0, 16)
+    free = kv.info()[1]
+    x = torch.zeros(8, device=DEV)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        x.add_(1)
+        st = torch.cuda.current_stream().cuda_stream
+        kv.reserve(0, 10, st)   # has them
+        for call in (lambda: kv.reserve(1, 16, st), lambda: kv.reserve(0, 17, st), lambda: kv.release(0, st)):
+            with pytest.raises(N.IllegalArgumentException):
+                call()
+    gr.replay()
+    torch.cuda.synchronize()
+    assert kv.info()[1] == free and bool((x == 1).all())
+    kv.reserve(1, 16)
+    assert kv.info()[1] == free - 1
