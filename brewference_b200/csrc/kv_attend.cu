@@ -16,8 +16,8 @@
 // moves only when exceeded by 2^2, so O is rarely rescaled.
 //
 // Work split.  Units of a tile for each warp of one (sequence, kv head, 8 pairs),
-// laid end to end over all sequences of the call; every CTA takes an equal
-// run of units, whatever the lengths (read on the device: a captured graph
+// laid end to end over all sequences of the call, each item's behind a weight;
+// every CTA takes an equal run, whatever the lengths (read on the device: a captured graph
 // follows them).  A run's first and last item may be shared with other CTAs:
 // their partial results (max, sum, O) go to the workspace and the last CTA to
 // arrive joins them in order.  Within an item each warp streams its own
@@ -53,6 +53,10 @@ constexpr int AT_FLUSH = 8;
 // kernel starts faster: one sequence of 300 positions with 256 pairs, 30 us
 // there, 23 here; of 4096 positions with 256 pairs 41 and 57, with 64 39 and 30.
 constexpr int64_t AT_PROMPT_PAIRS = 64, AT_PROMPT_PAIRS_FEW = 256, AT_MANY_PAIRS = 2048;
+// Units that an item weighs beside its own, for its start and end: without, the
+// CTAs that short sequences fall to are the last (32 sequences of 38 to 32768
+// positions, 28/4 heads of 128: 91 us, 80 with it).
+constexpr int AT_ITEM = 1;
 constexpr float AT_LAZY = 2.0f;                   // log2 of how far p may exceed 1
 
 template <int R>
@@ -183,7 +187,7 @@ __global__ void __launch_bounds__(AtShape<R>::THREADS, AtShape<R>::CTAS_PER_SM)
     auto entry_units = [&](const KvEntry& e) -> int64_t {
         if (e.rows <= 0 || (int64_t)e.rows * G >= p.pairs_min) return 0;
         const AtSpan sp = at_span<R>(e, p.window, G);
-        return (int64_t)sp.units * sp.groups * n_kv;
+        return (int64_t)(sp.units + AT_ITEM) * sp.groups * n_kv;
     };
     const int step = (n_seqs + S::THREADS - 1) / S::THREADS, nsteps = (n_seqs + step - 1) / step;
     int64_t U = 0;
@@ -226,14 +230,16 @@ __global__ void __launch_bounds__(AtShape<R>::THREADS, AtShape<R>::CTAS_PER_SM)
         for (int64_t n; k + 1 < n_seqs && rel >= (n = entry_units(e)); rel -= n) e = kv_check_entry(kv, p.rows, ++k);
         AtSpan sp = {0, 1, 1};
         if (e.rows > 0) sp = at_span<R>(e, p.window, G);
-        const int item = rel < (1ll << 31) ? (int)rel / sp.units : (int)(rel / sp.units);
+        const int width = sp.units + AT_ITEM;
+        const int item = rel < (1ll << 31) ? (int)rel / width : (int)(rel / width);
         s.seq = e.seq;
         s.pos0 = e.pos0;
         s.row0 = e.row0;
         s.units = sp.units;
-        s.ua = (int)(rel - (int64_t)item * sp.units);
-        s.ub = (int)min((int64_t)sp.units, s.ua + (u_end - u));
-        s.item0 = u - s.ua;
+        const int in = (int)(rel - (int64_t)item * width);   // below AT_ITEM: before the item's first unit
+        s.item0 = u - in + AT_ITEM;
+        s.ua = max(in - AT_ITEM, 0);
+        s.ub = (int)min((int64_t)sp.units, u_end - s.item0);
         s.hk = item / sp.groups;
         s.pr0 = (item - s.hk * sp.groups) * AT_PAIRS;
         s.npairs = (int)min((int64_t)e.rows * G - s.pr0, (int64_t)AT_PAIRS);
@@ -287,6 +293,7 @@ __global__ void __launch_bounds__(AtShape<R>::THREADS, AtShape<R>::CTAS_PER_SM)
     const AtSeg& done = s_done;
     locate(u_begin, seg);
     __syncwarp();
+    if (seg.ub <= seg.ua) return;   // nothing but an item's weight
     fill(seg);
     bool split_first = false, split_last = false;   // the run's first and last item is shared
 
@@ -538,10 +545,10 @@ __global__ void __launch_bounds__(AtShape<R>::THREADS, AtShape<R>::CTAS_PER_SM)
 
         // ---- the next item's first tiles, then this one's result
         const int64_t at = u;
-        u += seg.ub - seg.ua;
+        u = seg.item0 + seg.ub;
         if (tid == 0) s_done = seg;
         __syncwarp();
-        const bool more = u < u_end;
+        const bool more = u + AT_ITEM < u_end;
         if (more) {
             locate(u, seg);
             __syncwarp();
@@ -636,7 +643,7 @@ __global__ void __launch_bounds__(AtShape<R>::THREADS, AtShape<R>::CTAS_PER_SM)
     for (int x = 0; x < 2; ++x) {
         if (!s_join[x]) continue;
         const AtSeg& e = s_ends[x];
-        const bool first = U * c0[x] / C >= e.item0;   // the item is the first of CTA c0's run
+        const bool first = U * c0[x] / C >= e.item0 - AT_ITEM;   // the item is the first of CTA c0's run
         auto part = [&](int c) { return parts + (int64_t)((c0[x] + c) * 2 + (c == 0 && !first)) * at_part_floats(HD); };
         for (int r = warp; r < e.npairs; r += S::WARPS) {   // a warp for a pair
             float* wt = reinterpret_cast<float*>(ring);
