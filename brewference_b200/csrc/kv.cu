@@ -1,11 +1,12 @@
 // kv.cu — the paged 4-bit K/V cache: its handle (pages, reservations), the
 // append and read kernels and the C ABI of both and of the attention.
+#include <algorithm>
 #include <cmath>
 #include <new>
 #include <vector>
 
 #include "brew_internal.cuh"
-#include "kv.cuh"
+#include "kv_device.cuh"
 
 struct brew_kv_s {
     brew_kv_config c = {};
@@ -267,51 +268,68 @@ int append_r(const KvAppendParams& p, cudaStream_t s) {
 }
 
 // ---- read: the values that stored rows stand for --------------------------
-// One thread per 8 dims of a (row, kv head), k and v both: a word of k, two
-// halves of words of v.  Bound by the write of 4 bytes a value.
-constexpr int RD_ROWS = 4;
-
-__device__ __forceinline__ void kv_values(float* dst, uint32_t w, float d) {
-    float v[8];
+// 2^23 + code as the bits of a float, less 2^23 + 8, times d.
+__device__ __forceinline__ float4 kv_values4(uint32_t w, float d) {
+    float v[4];
 #pragma unroll
-    for (int c = 0; c < 8; ++c)   // 2^23 + code, as bits
-        v[c] = (__uint_as_float((w >> 4 * c & 15u) | 0x4B000000u) - 8388616.0f) * d;
-    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    for (int c = 0; c < 4; ++c) v[c] = (__uint_as_float((w >> 4 * c & 15u) | 0x4B000000u) - 8388616.0f) * d;
+    return make_float4(v[0], v[1], v[2], v[3]);
 }
 
-// A thread is 8 dims of a row and head.  Bound by its writes: 20 us for 5194
-// rows of 8 heads of 128, 42.6 MB, where the launch and the scattered words of
-// the codes take half.
+// A warp is 8 positions of a kv head, half a group, whose words it reads as
+// they lie: K's words are 8 dims of a position, V's 4 dims of two.  Bound by
+// the latency of entry, page and words one after the other: 16 us for 5194 rows
+// of 8 heads of 128 (42.6 MB written; 20 with 8 dims of a row a thread, which
+// gathers V's and the scales in 16-bit pieces).
 template <int R>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvView kv,
                                                       const __grid_constant__ KvRowsDev rows, float* k_out,
                                                       float* v_out, int64_t ld) {
     const KvEntry e = kv_entry(kv, rows, blockIdx.y, threadIdx.x == 0 && blockIdx.x == 0);
-    const int j0 = blockIdx.x * RD_ROWS, nr = min(RD_ROWS, e.rows - j0);
-    const int per = kv.n_kv * 4 * R;   // threads' work of a row
-    for (int x = threadIdx.x; x < nr * per; x += 256) {
-        const int r = x / per, t = x - r * per;
-        const int pos = e.pos0 + j0 + r, pg = pos & 15, u = pg >> 3;
-        const int hk = t / (4 * R), d8 = t % (4 * R), b = d8 / 4, i = d8 & 3;
-        const uint8_t* grp = kv_group<R>(kv, e.seq, pos, hk);
-        const int64_t o = ((int64_t)e.row0 + j0 + r) * ld + (int64_t)hk * 32 * R + 8 * d8;
-        const uint16_t* sc = reinterpret_cast<const uint16_t*>(grp + 512 * R);
-        const uint16_t* vq = reinterpret_cast<const uint16_t*>(grp + 256 * R);
-        const int half = pg & 1, at = (pg & 7) >> 1;
-        const uint32_t wk = reinterpret_cast<const uint32_t*>(grp)[kv_word(R, u, b, (pg & 7) * 4 + i)];
-        const uint32_t wv = vq[2 * kv_word(R, u, b, 8 * i + at) + half] |
-                            (uint32_t)vq[2 * kv_word(R, u, b, 8 * i + 4 + at) + half] << 16;
-        const float dk = half_bits_to_float(sc[kv_kscale(R, pg, b)]);
-        const float dv = half_bits_to_float(sc[16 * R + kv_vscale(R, pg, b)]);
-        if (k_out) kv_values(k_out + o, wk, dk);
-        if (v_out) kv_values(v_out + o, wv, dv);
+    if (e.rows <= 0) return;
+    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    const int first = e.pos0 >> 3, n = (((e.pos0 + e.rows - 1) >> 3) - first + 1) * kv.n_kv;
+    for (int x = blockIdx.x * 8 + (threadIdx.x >> 5); x < n; x += gridDim.x * 8) {
+        const int hk = x % kv.n_kv, base = (first + x / kv.n_kv) * 8, u = base >> 3 & 1;
+        const uint8_t* grp = kv_group<R>(kv, e.seq, base, hk);
+        const int64_t o = (int64_t)hk * 32 * R;
+        auto row = [&](int pos) { return (int64_t)(e.row0 + pos - e.pos0) * ld + o; };
+        auto in = [&](int pos) { return pos >= e.pos0 && pos < e.pos0 + e.rows; };
+        uint32_t wk[R], wv[R], dv[R];
+        __half dk[R];
+        if (k_out) load_words<R>(wk, grp, u, lane);
+        if (v_out) load_words<R>(wv, grp + 256 * R, u, lane);
+        if (k_out) load_kscales<R>(dk, grp + 512 * R, 8 * u + g);
+        if (v_out) load_scales<R>(dv, grp + 544 * R, u, q);
+        if (k_out && in(base + g)) {
+            float* at = k_out + row(base + g) + 8 * q;
+#pragma unroll
+            for (int b = 0; b < R; ++b) {
+                const float d = __half2float(dk[b]);
+                *reinterpret_cast<float4*>(at + 32 * b) = kv_values4(wk[b], d);
+                *reinterpret_cast<float4*>(at + 32 * b + 4) = kv_values4(wk[b] >> 16, d);
+            }
+        }
+        if (v_out) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int pos = base + 2 * q + h;
+                if (!in(pos)) continue;
+                float* at = v_out + row(pos) + 4 * g;
+#pragma unroll
+                for (int b = 0; b < R; ++b)
+                    *reinterpret_cast<float4*>(at + 32 * b) =
+                        kv_values4(wv[b] >> 16 * h, half_bits_to_float((uint16_t)(dv[b] >> 16 * h)));
+            }
+        }
     }
 }
 
 template <int R>
 int read_r(const KvView& kv, const KvRowsDev& rows, float* k, float* v, int64_t ld, cudaStream_t s) {
-    const dim3 grid((rows.max_rows + RD_ROWS - 1) / RD_ROWS, rows.n_seqs);
+    // positions of an entry begin anywhere in 8
+    const int64_t warps = ((int64_t)rows.max_rows + 14) / 8 * kv.n_kv;
+    const dim3 grid((unsigned)std::min<int64_t>((warps + 7) / 8, 1 << 16), rows.n_seqs);
     kv_read_kernel<R><<<grid, 256, 0, s>>>(kv, rows, k, v, ld);
     BREW_CUDA(cudaGetLastError());
     count_launch();
