@@ -17,7 +17,7 @@
 // The tiles of all items, end to end, are cut into one equal run a CTA, an
 // item's beginning and end (q, the output, a pipeline that empties) weighing 6
 // tiles (2: 156 us, 4: 126, 6: 117, 9: 118 for ragged prompts of up to 700
-// rows).  Items that a cut divides leave parts (O, maximum, sum) in the
+// rows, before the registers were divided as they are).  Items that a cut divides leave parts (O, maximum, sum) in the
 // workspace, which the last of their CTAs joins.
 //
 // 28 warps, the registers divided among them:
@@ -35,7 +35,7 @@
 //
 // Measured: a tile of 64 keys takes 1.4 us a CTA, where its 48 MMAs of 37
 // cycles take 1.0 (a chunk of 512 rows at 4096 positions, 16/8 heads of 128:
-// 64 us, of which 12 until the first product and 8 from the last to the joined
+// 62 us, of which 12 until the first product and 8 from the last to the joined
 // output).  What bounds it is the other warps' work beside them: 7800 warp
 // instructions a tile at 45% of the issue slots, in loops that have to stay in
 // the instruction cache together (the waits as a dozen instructions each, not
@@ -61,12 +61,16 @@ constexpr float PF_PLOG2 = 9.0f;       // p is carried times 2^9 (2^13 in tiles 
 constexpr int PF_QS = 36, PF_OS = 20;  // floats from row to row where q and the output are turned: no bank twice
 
 // Seven warpgroups; the first warp of each kind, and the registers of its
-// threads (the sum over the warpgroups is what the block is launched with).
+// threads (the sum over the warpgroups is what the block is launched with; 80
+// for the softmax and 64 for the unpacking: 64.5 us for the chunk below against
+// 61.7, 117 for the ragged prompts against 111).
 constexpr int PF_W_SOFT = 4, PF_W_SUM = 12, PF_W_UNPACK = 20, PF_THREADS = 896;
 constexpr int PF_ITEM_USERS = 3 + 24;   // warps that walk the run's items
-constexpr int PF_REGS = 72, PF_REGS_ISSUE = 40, PF_REGS_SOFT = 80, PF_REGS_SUM = 88, PF_REGS_UNPACK = 64;
+constexpr int PF_REGS = 72, PF_REGS_ISSUE = 40, PF_REGS_SOFT = 72, PF_REGS_SUM = 88, PF_REGS_UNPACK = 72;
 static_assert(PF_RAW <= 4, "rings of 4");
 static_assert(PF_REGS_ISSUE + 2 * (PF_REGS_SOFT + PF_REGS_SUM + PF_REGS_UNPACK) <= 7 * PF_REGS, "registers");
+static_assert(PF_REGS_ISSUE <= PF_REGS && PF_REGS_UNPACK <= PF_REGS && PF_REGS_SOFT >= PF_REGS && PF_REGS_SUM >= PF_REGS,
+              "the first two kinds give registers up, the others take some");
 
 // Tensor memory: S twice, O, q's parts, p's parts twice.
 constexpr uint32_t PF_T_S = 0, PF_T_O = 128, PF_T_QH = 256, PF_T_QL = 320, PF_T_P = 384;
