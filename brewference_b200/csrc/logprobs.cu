@@ -210,7 +210,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const __grid_co
         }
         __syncthreads();
     };
-    // the few logits before the first float4 and behind the last one
+    // the few logits before the first float4 and behind the last one; those behind it have the row's highest indexes, so
+    // they become candidates last (the list drops a later equal of its `top`-th)
     if (warp == 0 && (rank == 0 || rank == (uint32_t)cluster - 1)) {
         const int i = lane < 4 ? lane : head + 4 * quads + lane - 4;
         const bool is = lane < 8 && (lane < 4 ? rank == 0 && lane < head : rank == (uint32_t)cluster - 1 && i < p.vocab);
@@ -218,7 +219,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const __grid_co
         raise(v);
         if (is && s.r == -INFINITY) s.z += v - v == 0.0f || v == -INFINITY ? 0.0f : v - v;   // a NaN alone
         else if (is) add(v);
-        if (TOP && is) {
+        if (TOP && is && lane < 4) {
             const float c[4] = {v, 0, 0, 0};
             append(c, 1, i);
         }
@@ -282,7 +283,14 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const __grid_co
             }
         }
     }
-    if (TOP) take();
+    if (TOP) {
+        const int i = head + 4 * quads + lane;
+        if (warp == 0 && rank == (uint32_t)cluster - 1 && lane < 4 && i < p.vocab) {
+            const float c[4] = {x[i], 0, 0, 0};
+            append(c, 1, i);
+        }
+        take();
+    }
 
     // ---- joins: lanes, warps, CTAs
 #pragma unroll
