@@ -12,7 +12,10 @@
 //   output   O = sum_t (p_t d_V[t][b]) (c_ti - 8)
 // q, p and d_V are scaled by powers of two (q below 2^14, p and p d_V to 2^15
 // at most), so that no part leaves fp16's range and little falls among its
-// subnormals (2^-24 beside 2^13).  The softmax is online; its running maximum
+// subnormals (2^-24 beside 2^13): each block of V has a power of its own, at
+// least 1, so that no d_V is rounded for another block or another tile; where p
+// d_V would pass 2^15 all the same (values over 32 that carry the weight), the
+// tile's p are taken down instead.  The softmax is online; its running maximum
 // moves only when exceeded by 2^2, so O is rarely rescaled.
 //
 // Work split.  Units of a tile for each warp of one (sequence, kv head, 8 pairs),
@@ -97,23 +100,21 @@ __device__ __forceinline__ void mma_f16_new(float (&d)[4], const uint32_t (&a)[4
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The power of two that d_V is carried with, from the exponent over every
-// |d_V| so far (|d_V| < 2^(ve - 15)): scales all under 2^-6, and those that
-// reach 1, are brought to about 1, so that p d_V times both factors stays
-// under 2^15 and its small terms off fp16's subnormals.
 constexpr float AT_PLOG2 = 13.0f;   // p is carried times 2^13, sums and all: p may be 2^AT_LAZY
-struct AtScale {
-    uint32_t ve;     // 1 .. 32
-    uint32_t dmul;   // factor of d_V, an fp16 pair
-    float total;     // the same, fp32
-    __device__ explicit AtScale(uint32_t e) : ve(e) {
-        const int up = e < 10 || e > 15 ? 15 - (int)e : 0;
-        // 2^-15 and less (d_V at fp16's end) are subnormals
-        const uint32_t h = up > -15 ? (uint32_t)(15 + up) << 10 : 1u << (25 + up - 1);
-        dmul = h | h << 16;
-        total = __uint_as_float((uint32_t)(127 + up) << 23);
-    }
-};
+// A block's d_V are carried times 2^up, up >= 0, which brings the largest of them
+// under 1, and over 2^-6 or so: above, p d_V might pass fp16; below, its second
+// part would lie among the subnormals.  It moves when a tile's scales leave
+// [2^-8, 1]: they differ little from tile to tile, so that is rare.  The blocks'
+// ups are the nibbles of a register.  (One power for all blocks, from the largest
+// so far, rounded d_V themselves: 60 % off in a block 10^7 below another.  The
+// check costs 1 % of a batch, 188.3 us against 186.2.)
+constexpr int AT_UP_MAX = 14;       // 2^14 is about where fp16 ends
+__device__ __forceinline__ int up_of(uint32_t ups, int b) { return (int)(ups >> 4 * b & 15u); }
+__device__ __forceinline__ uint32_t up_h2(uint32_t ups, int b) {
+    const uint32_t h = (uint32_t)(15 + up_of(ups, b)) << 10;
+    return h | h << 16;
+}
+__device__ __forceinline__ float pow2f(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
 
 // An 8 x 8 matrix of fp16, row g in lanes 4 g .. 4 g + 3, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -379,9 +380,20 @@ __global__ void __launch_bounds__(AtShape<R>::THREADS, AtShape<R>::CTAS_PER_SM)
                     for (int c = 0; c < 4; ++c) o[b][t][c] *= k[c & 1];
             if (kept) keep(k);
         };
+        auto lower = [&](int sign, int k) {   // o = o * 2^(sign * k), k of the pair's own lanes
+            float f[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) f[c] = pow2f(sign * __shfl_sync(0xffffffffu, k, 8 * i + 4 * c));
+#pragma unroll
+            for (int b = 0; b < R; ++b)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) o[b][t][c] *= f[c & 1];
+        };
         float m[2] = {-INFINITY, -INFINITY};
         float2 l2 = make_float2(0.0f, 0.0f);
-        AtScale sv(1);
+        uint32_t ups = 0;
 
         for (int k = 0; k < seg.nt; ++k) {
             const uint32_t slot = nth % S::STAGES;
@@ -481,25 +493,86 @@ __global__ void __launch_bounds__(AtShape<R>::THREADS, AtShape<R>::CTAS_PER_SM)
             }
 
             // ---- O += (p d_V) (c - 8), a group of 16 positions at a time
-            uint32_t dm = 0;
-#pragma unroll
-            for (int u4 = 0; u4 < 4; ++u4)
-#pragma unroll
-                for (int b = 0; b < R; ++b) dm = maxabs_h2(dm, vsc[u4][b]);
+            int down = 0;          // log2 of what this lane's pair's p are divided by for this tile
+            bool lowered = false;  // some pair's are
             {
-                const uint32_t top = max(dm & 0x7FFFu, dm >> 16 & 0x7FFFu) >> 10;   // fp16's exponent field
-                if (__any_sync(0xffffffffu, top >= sv.ve)) {
-                    const AtScale next(__reduce_max_sync(0xffffffffu, top) + 1);
-                    float corr[2];
-                    corr[0] = corr[1] = next.total * (1.0f / sv.total);
-                    sv = next;
-                    rescale(corr);
+                uint32_t hi = 0, lo = 0x7C007C00u;   // the blocks' largest scales: the largest and the smallest
+#pragma unroll
+                for (int b = 0; b < R; ++b) {
+                    const uint32_t d = maxabs_h2(maxabs_h2(vsc[0][b], vsc[1][b]), maxabs_h2(vsc[2][b], vsc[3][b]));
+                    hi = maxabs_h2(hi, d);
+                    lo = minabs_h2(lo, d);
                 }
-                if (sv.dmul != 0x3C003C00u) {
+                if (__builtin_expect(ups != 0, 0)) {
+                    hi = 0;
+                    lo = 0x7C007C00u;
 #pragma unroll
-                    for (int u4 = 0; u4 < 4; ++u4)
+                    for (int b = 0; b < R; ++b) {
+                        const uint32_t d = mul_h2(maxabs_h2(maxabs_h2(vsc[0][b], vsc[1][b]), maxabs_h2(vsc[2][b], vsc[3][b])), up_h2(ups, b));
+                        hi = maxabs_h2(hi, d);
+                        lo = minabs_h2(lo, d);
+                    }
+                }
+                // in either half: hi over 1 (0x3C00, to which 0x43FF carries) or lo under 2^-8 (0x1C00, 0x6400)
+                const uint32_t out = ((hi & 0x7FFF7FFFu) + 0x43FF43FFu) | ~((lo & 0x7FFF7FFFu) + 0x64006400u);
+                if (__builtin_expect(__any_sync(0xffffffffu, out & 0x80008000u), 0)) {
 #pragma unroll
-                        for (int b = 0; b < R; ++b) vsc[u4][b] = mul_h2(vsc[u4][b], sv.dmul);
+                    for (int b = 0; b < R; ++b) {
+                        const uint32_t d = maxabs_h2(maxabs_h2(vsc[0][b], vsc[1][b]), maxabs_h2(vsc[2][b], vsc[3][b])) & 0x7FFF7FFFu;
+                        const uint32_t d0 = d & 0xFFFFu, d1 = d >> 16;   // (NaN: no size)
+                        const uint32_t top = __reduce_max_sync(0xffffffffu, max(d0 < 0x7C00u ? d0 : 0u, d1 < 0x7C00u ? d1 : 0u));
+                        const int k = up_of(ups, b), e = (int)(top >> 10) - 14 + k;   // top * 2^up < 2^e
+                        const int next = top != 0 && (e > 0 || e < -5) ? min(AT_UP_MAX, max(0, k - e)) : k;
+                        if (next != k) {
+                            const float f = pow2f(next - k);
+#pragma unroll
+                            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) o[b][t][c] *= f;
+                            if (kept) {
+                                float4* sm = reinterpret_cast<float4*>(mine);
+#pragma unroll
+                                for (int t = 0; t < 2; ++t) {
+                                    float4 v = sm[(2 * b + t) * 32 + lane];
+                                    v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+                                    sm[(2 * b + t) * 32 + lane] = v;
+                                }
+                            }
+                            ups ^= (uint32_t)(k ^ next) << 4 * b;
+                        }
+                    }
+                    // the pair's largest p d_V: 2^15 at most
+                    float most = 0.0f;
+#pragma unroll
+                    for (int u4 = 0; u4 < 4; ++u4) {
+                        const uint32_t pt = transpose8(pack_half2(s[u4 >> 1][2 * (u4 & 1)], s[u4 >> 1][2 * (u4 & 1) + 1]));
+                        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&pt));
+#pragma unroll
+                        for (int b = 0; b < R; ++b) {
+                            const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&vsc[u4][b]));
+                            most = fmaxf(most, fmaxf(fabsf(x.x * d.x), fabsf(x.y * d.y)) * pow2f(up_of(ups, b)));
+                        }
+                    }
+#pragma unroll
+                    for (int w = 1; w < 4; w <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
+                    if (most > 32768.0f) down = (int)(__float_as_uint(most) >> 23) - 127 - 14;
+                    lowered = __any_sync(0xffffffffu, down > 0);
+                    if (lowered) {
+                        const float f[2] = {pow2f(-__shfl_sync(0xffffffffu, down, 8 * i)), pow2f(-__shfl_sync(0xffffffffu, down, 8 * i + 4))};
+#pragma unroll
+                        for (int gr = 0; gr < 2; ++gr)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) s[gr][c] *= f[c & 1];
+                        lower(-1, down);
+                    }
+                }
+                if (__builtin_expect(ups != 0, 0)) {
+#pragma unroll
+                    for (int b = 0; b < R; ++b) {
+                        const uint32_t f = up_h2(ups, b);
+#pragma unroll
+                        for (int u4 = 0; u4 < 4; ++u4) vsc[u4][b] = mul_h2(vsc[u4][b], f);
+                    }
                 }
             }
 #pragma unroll
@@ -531,6 +604,7 @@ __global__ void __launch_bounds__(AtShape<R>::THREADS, AtShape<R>::CTAS_PER_SM)
                     }
                 }
             }
+            if (__builtin_expect(lowered, 0)) lower(1, down);
             __syncwarp();   // every lane has read the stage
             if (k + S::STAGES < seg.nt) {
                 if (((k + S::STAGES) & 31) == 0) lookup(seg, k + S::STAGES);
@@ -571,13 +645,14 @@ __global__ void __launch_bounds__(AtShape<R>::THREADS, AtShape<R>::CTAS_PER_SM)
                     }
                 __syncwarp();
             }
-            const float un = 1.0f / sv.total;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
 #pragma unroll
-                for (int b = 0; b < R; ++b)
+                for (int b = 0; b < R; ++b) {
+                    const float un = pow2f(-up_of(ups, b));
                     *reinterpret_cast<float4*>(mine + (2 * i + c) * S::PITCH + 32 * b + 4 * g) =
                         make_float4(o[b][0][c] * un, o[b][0][c + 2] * un, o[b][1][c] * un, o[b][1][c + 2] * un);
+                }
                 if (g == 0) {
                     mine[AT_PAIRS * S::PITCH + 2 * (2 * i + c)] = m[c];
                     mine[AT_PAIRS * S::PITCH + 2 * (2 * i + c) + 1] = l[c];

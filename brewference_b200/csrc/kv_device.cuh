@@ -74,6 +74,13 @@ __device__ __forceinline__ uint32_t maxabs_h2(uint32_t a, uint32_t b) {
     return d;
 }
 
+// The smaller one.
+__device__ __forceinline__ uint32_t minabs_h2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("min.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
