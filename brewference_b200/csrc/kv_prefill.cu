@@ -347,6 +347,27 @@ __device__ __forceinline__ bool pf_q_store(const KvAttendParams& p, PfRest& sh, 
     return true;
 }
 
+// A tile with a scale over 8188, or a NaN: bit 16, whether it is one that some
+// row sees, and a number; below, the positions of group w with a NaN among V's.
+template <int R>
+__device__ __noinline__ uint32_t pf_rare(const uint8_t* tile, int k0, int kmin, int kmax, int w, int lane) {
+    uint32_t seen = 0;
+#pragma unroll 1
+    for (int z = lane; z < PF_GROUPS * 16 * R; z += 32) {
+        const int y = z / (16 * R), n = z % (16 * R);   // words of a group: 8 R of K's, 8 R of V's
+        const uint32_t d = reinterpret_cast<const uint32_t*>(tile + y * kv_group_bytes(R) + 512 * R)[n] & 0x7FFF7FFFu;
+        const int p0 = k0 + 16 * y + (n < 8 * R ? 2 * n / R : (n - 8 * R) / R * 2), p1 = n < 8 * R ? p0 : p0 + 1;
+        const uint32_t d0 = d & 0xFFFFu, d1 = d >> 16;
+        if (p0 >= kmin && p0 <= kmax && d0 < 0x7C00u) seen = max(seen, d0);
+        if (p1 >= kmin && p1 <= kmax && d1 < 0x7C00u) seen = max(seen, d1);
+    }
+    bool nan = false;   // lane = position
+#pragma unroll 1
+    for (int y = 0; y < R && k0 + 16 * w <= kmax; ++y)
+        nan |= (reinterpret_cast<const uint16_t*>(tile + w * kv_group_bytes(R) + 544 * R)[kv_vscale(R, lane & 15, y)] & 0x7FFFu) > 0x7C00u;
+    return (__reduce_max_sync(0xffffffffu, seen) > 0x6FFFu ? 0x10000u : 0u) | (__ballot_sync(0xffffffffu, nan) & 0xFFFFu);
+}
+
 template <int R>
 __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_constant__ KvAttendParams p) {
     using S = PfShape<R>;
@@ -922,8 +943,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
                     ok = pf_wait_warp(&sh.raw_full[st], i / PF_RAW & 1, kv.err);
                     if (!ok) break;
                     if (is_k) {
-                        // the largest scale of the tile's live groups (as fp16 bits): above 8188 its values are taken times
-                        // 2^-4, so that d (c - 8) stays in fp16's range; above infinity some are NaN
+                        // The largest scale of the tile's live groups (as fp16 bits): above 8188 its values are taken times
+                        // 2^-4, so that d (c - 8) stays in fp16's range; above infinity some are NaN.  (2^-4 rounds scales
+                        // under 2^-10 to multiples of 2^-20: beside a value past 65504 that some row of the item sees.)
                         uint32_t top = 0;
 #pragma unroll
                         for (int y = 0; y < PF_GROUPS; ++y)
@@ -933,15 +955,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
                                     top = __vmaxu2(top, reinterpret_cast<const uint32_t*>(tile + y * kv_group_bytes(R) + 512 * R)[z] &
                                                             0x7FFF7FFFu);
                         top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
-                        const bool big = top > 0x6FFFu;
-                        uint32_t nan = 0;
-                        if (top > 0x7C00u && k0 + 16 * w <= x.kmax) {
-                            bool mine = false;   // lane = position
-#pragma unroll
-                            for (int y = 0; y < R; ++y)
-                                mine |= (reinterpret_cast<const uint16_t*>(raw + 544 * R)[kv_vscale(R, lane & 15, y)] & 0x7FFFu) > 0x7C00u;
-                            nan = __ballot_sync(0xffffffffu, mine) & 0xFFFFu;
-                        }
+                        uint32_t rare = 0;   // bit 16: some value is past fp16; below: V's positions with a NaN
+                        if (top > 0x6FFFu) rare = pf_rare<R>(tile, k0, x.kmin, x.kmax, w, lane);
+                        const bool big = rare >> 16;
+                        const uint32_t nan = rare & 0xFFFFu;
                         ok = pf_wait_warp(&sh.k_empty[b], (i >> 1 & 1) ^ 1, kv.err);
                         if (!ok) break;
                         if (lane == 0) {
