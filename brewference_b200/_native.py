@@ -145,6 +145,7 @@ def lib():
                                       ctypes.POINTER(I64)]),
         "brew_model_load_gguf": (I, [ctypes.c_char_p, ctypes.c_int32, c_void_pp]),
         "brew_selftest_wait_timeout": (I, [I64, c_i32p]),
+        "brew_selftest_raise_counters": (I, [V]),
         "brew_model_set_kv_cache": (I, [V, ctypes.c_int32]),
         "brew_session_score": (I, [V, c_i32p, ctypes.c_int32, ctypes.c_int32, c_f32p, c_f32p, c_i32p, c_f32p]),
         "brew_kv_create": (I, [ctypes.POINTER(KvConfig), c_void_pp]),

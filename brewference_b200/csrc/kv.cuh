@@ -96,6 +96,9 @@ int kv_clear(brew_kv_s* kv, cudaStream_t s);
 int kv_append_launch(int head_size, const KvAppendParams& p, cudaStream_t s);
 int kv_attend_launch(int head_size, const KvAttendParams& p, cudaStream_t s);
 int64_t kv_attend_workspace(int head_size);
+// The workspace's arrival counters set to `value` bytes in stream order: 0 makes it ready again after a call that a
+// bounded wait ended.
+int kv_attend_counters(int head_size, void* workspace, int value, cudaStream_t s);
 bool kv_head_supported(int head_size);
 // The prompt kernel (tcgen05), its part of the workspace: kv_attend_launch's.
 constexpr int KV_COUNTER_BYTES = 4096;

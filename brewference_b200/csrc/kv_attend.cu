@@ -799,6 +799,13 @@ static int64_t at_workspace(int head_size) {
 }
 int64_t kv_attend_workspace(int head_size) { return at_workspace(head_size) + kv_prefill_workspace(head_size); }
 
+int kv_attend_counters(int hd, void* workspace, int value, cudaStream_t s) {
+    uint8_t* w = static_cast<uint8_t*>(workspace);
+    BREW_CUDA(cudaMemsetAsync(w, value, KV_COUNTER_BYTES, s));
+    if (kv_prefill_supported(hd)) BREW_CUDA(cudaMemsetAsync(w + at_workspace(hd), value, KV_COUNTER_BYTES, s));
+    return BREW_OK;
+}
+
 int kv_attend_launch(int hd, const KvAttendParams& p0, cudaStream_t s) {
     KvAttendParams p = p0;
     const int64_t most = (int64_t)p.rows.max_rows * (p.kv.n_heads / p.kv.n_kv);

@@ -1378,6 +1378,10 @@ int after_step_check(brew_model_s* m, const char* where) {
         cudaMemset(m->am_ctr, 0, (size_t)m->max_batch * sizeof(int));
         cudaDeviceSynchronize();
     }
+    if (rc && m->kv_ws) {   // an attention whose wait ended has not met its other parts
+        kv_attend_counters(m->c.head_size, m->kv_ws, 0, ctx().stream);
+        cudaDeviceSynchronize();
+    }
     return rc;
 }
 
@@ -1746,6 +1750,16 @@ int brew_model_set_kv_cache(brew_model m, int32_t type) {
     return BREW_OK;
 }
 
+int brew_selftest_raise_counters(brew_model m) {
+    BREW_CHECK(m && m->kv, BREW_ERR_INVALID_ARG, "a model with a 4-bit K/V cache is wanted");
+    int rc = ensure_init();
+    if (rc) return rc;
+    std::lock_guard<std::mutex> lk(api_mutex());
+    if ((rc = kv_attend_counters(m->c.head_size, m->kv_ws, 1, ctx().stream))) return rc;
+    BREW_CUDA(cudaStreamSynchronize(ctx().stream));
+    return BREW_OK;
+}
+
 int brew_session_score(brew_model m, const int32_t* tokens, int32_t n, int32_t top, float* logprob, float* entropy,
                        int32_t* top_ids, float* top_logprobs) {
     BREW_CHECK(m && tokens, BREW_ERR_INVALID_ARG, "null argument");
@@ -1829,7 +1843,10 @@ int brew_model_set_trace(brew_model m, int32_t on) {
 int brew_model_reset(brew_model m) {
     BREW_CHECK(m, BREW_ERR_INVALID_ARG, "null model");
     std::lock_guard<std::mutex> lk(api_mutex());
-    if (m->kv) return kv_clear(m->kv, ctx().stream);
+    if (m->kv) {
+        const int rc = kv_attend_counters(m->c.head_size, m->kv_ws, 0, ctx().stream);
+        return rc ? rc : kv_clear(m->kv, ctx().stream);
+    }
     BREW_CUDA(cudaMemsetAsync(m->kc, 0, (size_t)m->max_batch * m->cache_bstride * sizeof(float), ctx().stream));
     BREW_CUDA(cudaMemsetAsync(m->vc, 0, (size_t)m->max_batch * m->cache_bstride * sizeof(float), ctx().stream));
     BREW_CUDA(cudaStreamSynchronize(ctx().stream));

@@ -409,6 +409,10 @@ BREW_API int brew_model_trace(brew_model m, int64_t* ns, int32_t max_n, int32_t*
  * ended as designed; *waits_ended (optional) receives how many did (2).
  * The context stays usable afterwards. */
 BREW_API int brew_selftest_wait_timeout(int64_t limit_ns, int32_t* waits_ended);
+/* Leaves the arrival counters of a 4-bit-cache model's attention raised, as a
+ * step that a bounded wait ended may: the next call that reports a device
+ * error, and brew_model_reset, have to put them back. */
+BREW_API int brew_selftest_raise_counters(brew_model m);
 
 /* ---- paged 4-bit K/V cache ------------------------------------------------
  * No reference counterpart: its RunState keeps fp32 K and V of seq_len
@@ -500,7 +504,7 @@ BREW_API int brew_kv_read_dev(brew_kv kv, int32_t layer, float* k_out, float* v_
  * 0); scale 0 means 1 / sqrt(head_size).  out may not overlap q.  `workspace`:
  * brew_kv_workspace_bytes(kv) device bytes on a 256-byte boundary,
  * zero-filled once before its first use (each call leaves it ready for the
- * next, unless brew_kv_check reports BREW_ERR_TIMEOUT).  Calls and captured
+ * next, unless brew_kv_check reports BREW_ERR_TIMEOUT: zero-fill it again then).  Calls and captured
  * graphs that may run at the same time need a workspace each.  Positions that
  * a row does not see may hold anything.  A stored NaN makes the outputs that
  * depend on it NaN (a key's: the row's whole head; a value's: its block of 32
