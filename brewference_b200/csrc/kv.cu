@@ -515,7 +515,9 @@ int brew_kv_reserve(brew_kv kv, int32_t seq, int32_t n_tokens, void* stream) {
         have.push_back(kv->free_pages.back());
         kv->free_pages.pop_back();
     }
-    rc = set_pages(kv, seq, first, need, (int)(need << kv->page_shift), static_cast<cudaStream_t>(stream));
+    // the last page may reach past max_tokens: the sequence does not
+    const int tokens = (int)std::min<size_t>(need << kv->page_shift, kv->c.max_tokens);
+    rc = set_pages(kv, seq, first, need, tokens, static_cast<cudaStream_t>(stream));
     for (; rc && have.size() > first; have.pop_back()) kv->free_pages.push_back(have.back());
     return rc;
 }

@@ -425,8 +425,8 @@ BREW_API int brew_selftest_raise_counters(brew_model m);
  *
  * brew_kv_reserve gives sequence `seq` the pages of positions 0 ..
  * n_tokens - 1 (it only grows; BREW_ERR_CONTEXT_FULL past max_tokens or when
- * the pool is empty, nothing is changed then), brew_kv_release returns them
- * all.  Both take effect on the device in `stream` order; a page released on
+ * the pool is empty, nothing is changed then); the rest of the last page can
+ * be used too, up to max_tokens.  brew_kv_release returns them all.  Both take effect on the device in `stream` order; a page released on
  * one stream and taken on another needs an ordering between the two.  Neither
  * can be captured into a CUDA graph (BREW_ERR_INVALID_ARG).
  *

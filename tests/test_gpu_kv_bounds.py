@@ -1,0 +1,64 @@
+"""Where a sequence of the paged 4-bit K/V cache ends."""
+import pytest
+import torch
+
+from brewference_b200 import _native as N
+from brewference_b200 import config as C
+from brewference_b200.api import DeviceModel
+from test_gpu_kv import DEV, Filled, i32, make_rows
+from test_gpu_model import small
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_a_sequence_ends_at_max_tokens(device, page):
+    """Not where its last page ends."""
+    f = Filled(4, 2, 64, [100, 60], page, seed=1, max_tokens=100, spare=9)
+    f.check(f.q(2), [(0, 99, 1), (1, 59, 1)])
+    k = torch.randn(3, 2, 64, generator=f.g, device=DEV)
+    for seq, pos, n in ((0, 100, 1), (0, 98, 3), (0, page * (99 // page + 1) - 1, 1)):
+        rows = make_rows([(seq, pos, n)])
+        f.kv.append(0, 0, 0, 0, k.data_ptr(), k.data_ptr(), 128, rows)
+        with pytest.raises(N.IllegalStateException):
+            f.kv.check()
+        out = torch.full((3, 2, 64), 3.0, device=DEV)
+        f.kv.read(0, out.data_ptr(), 0, 128, rows)
+        with pytest.raises(N.IllegalStateException):
+            f.kv.check()
+        assert bool((out == 3).all())
+        assert torch.isnan(f.attend(f.q(n), [(seq, pos, n)])).all()
+        with pytest.raises(N.IllegalStateException):
+            f.kv.check()
+    # pages are given whole: what is reserved is usable up to the page's end, and no further
+    end = min(100, page * (59 // page + 1))
+    f.kv.append(0, 0, 0, 0, k.data_ptr(), k.data_ptr(), 128, make_rows([(1, end - 1, 1)]))
+    f.kv.check()
+    f.kv.reserve(1, 100)
+    f.kv.append(0, 0, 0, 0, k.data_ptr(), k.data_ptr(), 128, make_rows([(1, 97, 3)]))
+    f.kv.check()
+    f.kv.append(0, 0, 0, 0, k.data_ptr(), k.data_ptr(), 128, make_rows([(1, 98, 3)]))
+    with pytest.raises(N.IllegalStateException):
+        f.kv.check()
+
+
+@pytest.mark.parametrize("qtype", [C.TYPE_F32, C.TYPE_Q4_0])
+def test_a_models_sequence_ends_at_its_context(device, qtype):
+    """Positions given on the device, past the 100 of the context."""
+    dm = DeviceModel.synthesize(small(C.ARCH_QWEN3, seq_len=100), 3, max_batch=2)
+    dm.set_kv_cache(qtype)
+    tok, am = i32([5, 6]), i32([0, 0])
+
+    def step(pos):
+        p = i32(pos)
+        torch.cuda.synchronize()
+        N.check(N.lib().brew_model_forward_dev(dm.handle, tok.data_ptr(), p.data_ptr(), 2, None, am.data_ptr(), None))
+        torch.cuda.synchronize()
+
+    step([99, 99])
+    dm.forward([1, 2], [0, 0])
+    step([99, 100])
+    with pytest.raises(N.IllegalStateException):   # told by the next call that checks
+        dm.forward([1, 2], [0, 0])
+    dm.forward([1, 2], [0, 0])
+    dm.close()
