@@ -26,30 +26,28 @@ struct brew_kv_s {
 namespace brew {
 namespace {
 
-// Page ids of positions first .. first + n - 1 pages of a sequence, and then
-// its reserved positions: launch parameters, so that the call stays
-// asynchronous and needs no staging buffer.
+// Page ids of a sequence, and then its reserved positions: launch parameters,
+// so that the call stays asynchronous and needs no staging buffer.
 struct KvIds {
-    int32_t id[120];
+    int32_t id[KV_PUT_PAGES];
 };
 
 __global__ void kv_table_kernel(int32_t* row, int first, int n, KvIds ids, int32_t* reserved, int tokens) {
     if ((int)threadIdx.x < n) row[first + threadIdx.x] = ids.id[threadIdx.x];
-    if (threadIdx.x == 0) *reserved = tokens;
+    if (threadIdx.x == 0 && tokens >= 0) *reserved = tokens;
 }
 
-int set_pages(brew_kv_s* kv, int seq, size_t first, size_t end, int tokens, cudaStream_t s) {
+int set_pages(brew_kv_s* kv, int seq, int first, int end, int tokens, cudaStream_t s) {
     const std::vector<int32_t>& pages = kv->seq_pages[seq];
     int32_t* row = kv->table + (int64_t)seq * kv->max_pages;
     do {
+        const KvPut p = kv_put(first, end, tokens);
         KvIds ids;
-        const int n = (int)std::min<size_t>(end - first, 120);
-        for (int i = 0; i < n; ++i) ids.id[i] = pages[first + i];
-        const int now = (size_t)n == end - first ? tokens : (int)((first + n) << kv->page_shift);
-        kv_table_kernel<<<1, 128, 0, s>>>(row, (int)first, n, ids, kv->reserved + seq, now);
+        for (int i = 0; i < p.n; ++i) ids.id[i] = pages[first + i];
+        kv_table_kernel<<<1, 128, 0, s>>>(row, first, p.n, ids, kv->reserved + seq, p.tokens);
         BREW_CUDA(cudaGetLastError());
         count_launch();
-        first += n;
+        first += p.n;
     } while (first < end);
     return BREW_OK;
 }
@@ -517,7 +515,7 @@ int brew_kv_reserve(brew_kv kv, int32_t seq, int32_t n_tokens, void* stream) {
     }
     // the last page may reach past max_tokens: the sequence does not
     const int tokens = (int)std::min<size_t>(need << kv->page_shift, kv->c.max_tokens);
-    rc = set_pages(kv, seq, first, need, tokens, static_cast<cudaStream_t>(stream));
+    rc = set_pages(kv, seq, (int)first, (int)need, tokens, static_cast<cudaStream_t>(stream));
     for (; rc && have.size() > first; have.pop_back()) kv->free_pages.push_back(have.back());
     return rc;
 }

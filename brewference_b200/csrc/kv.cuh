@@ -41,6 +41,19 @@ __host__ __device__ constexpr int kv_word(int R, int u, int b, int lane) {
 __host__ __device__ constexpr int kv_kscale(int R, int p, int b) { return p * R + b; }
 __host__ __device__ constexpr int kv_vscale(int R, int p, int b) { return ((p >> 1) * R + b) * 2 + (p & 1); }
 
+// One launch of a reservation: page ids first .. first + n - 1 of a sequence,
+// and its reserved positions, or -1 where more launches follow: the length is
+// published behind its last page id, so that one whose launches fail midway
+// leaves the old one in force (its pages may be another sequence's by then).
+constexpr int KV_PUT_PAGES = 120;
+struct KvPut {
+    int first, n, tokens;
+};
+inline KvPut kv_put(int first, int end, int tokens) {
+    const int n = end - first < KV_PUT_PAGES ? end - first : KV_PUT_PAGES;
+    return {first, n, first + n == end ? tokens : -1};
+}
+
 // The cache as the kernels see it, one layer.
 struct KvView {
     uint8_t* pages;            // [n_pages][n_kv][page_tokens / 16] groups

@@ -4,8 +4,8 @@ import torch
 
 from brewference_b200 import _native as N
 from brewference_b200 import config as C
-from brewference_b200.api import DeviceModel
-from test_gpu_kv import DEV, Filled, i32, make_rows
+from brewference_b200.api import DeviceModel, KvCache
+from test_gpu_kv import DEV, Filled, i32, make_rows, stored
 from test_gpu_model import small
 
 pytestmark = pytest.mark.gpu
@@ -40,6 +40,22 @@ def test_a_sequence_ends_at_max_tokens(device, page):
     f.kv.append(0, 0, 0, 0, k.data_ptr(), k.data_ptr(), 128, make_rows([(1, 98, 3)]))
     with pytest.raises(N.IllegalStateException):
         f.kv.check()
+
+
+def test_a_reservation_of_many_launches(device):
+    """Pages past the 120 that one launch hands over, given in three steps."""
+    kv = KvCache(1, 2, 1, 32, 2, 5003, 16, 0)
+    k = torch.randn(5003, 1, 32, device=DEV)
+    out = torch.empty_like(k)
+    for n in (1900, 3900, 5003):
+        kv.reserve(1, n)
+        kv.append(0, 0, 0, 0, k.data_ptr(), k.data_ptr(), 32, make_rows([(1, 0, n)]))
+        kv.read(0, out.data_ptr(), 0, 32, make_rows([(1, 0, n)]))
+        kv.check()
+        assert torch.equal(out[:n], stored(k[:n]).float())
+    kv.append(0, 0, 0, 0, k.data_ptr(), k.data_ptr(), 32, make_rows([(1, 5003, 1)]))
+    with pytest.raises(N.IllegalStateException):
+        kv.check()
 
 
 @pytest.mark.parametrize("qtype", [C.TYPE_F32, C.TYPE_Q4_0])
