@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(const __grid_cons
 
 template <int R>
 int append_r(const KvAppendParams& p, cudaStream_t s) {
-    const dim3 grid((p.rows.max_rows + AP_ROWS - 1) / AP_ROWS, p.rows.n_seqs);
+    const dim3 grid((unsigned)(((int64_t)p.rows.max_rows + AP_ROWS - 1) / AP_ROWS), p.rows.n_seqs);
     auto go = [&](auto kernel) { kernel<<<grid, AP_THREADS, 0, s>>>(p); };
     if (p.qnorm || p.knorm) {
         if (p.rope == BREW_KV_ROPE_HALF) go(kv_append_kernel<R, true, BREW_KV_ROPE_HALF>);
@@ -362,8 +362,9 @@ int check_matrix(const char* what, const void* p, int64_t ld, int64_t width) {
     return BREW_OK;
 }
 
+// (an entry has no more rows than the buffers: grids do not grow with a bound far above them)
 KvRowsDev rows_dev(const brew_kv_rows* r) {
-    return {r->seq, r->pos, r->row_start, r->n_seqs, r->n_rows, r->max_rows};
+    return {r->seq, r->pos, r->row_start, r->n_seqs, r->n_rows, std::min(r->max_rows, r->n_rows)};
 }
 
 }  // namespace

@@ -1,10 +1,11 @@
-"""Where a sequence of the paged 4-bit K/V cache ends."""
+"""Where a sequence of the paged 4-bit K/V cache ends, and how many rows a
+call may say an entry has."""
 import pytest
 import torch
 
 from brewference_b200 import _native as N
 from brewference_b200 import config as C
-from brewference_b200.api import DeviceModel, KvCache
+from brewference_b200.api import DeviceModel, KvCache, KvRows
 from test_gpu_kv import DEV, Filled, i32, make_rows, stored
 from test_gpu_model import small
 
@@ -78,3 +79,22 @@ def test_a_models_sequence_ends_at_its_context(device, qtype):
         dm.forward([1, 2], [0, 0])
     dm.forward([1, 2], [0, 0])
     dm.close()
+
+
+@pytest.mark.parametrize("max_rows", [2 ** 31 - 1, 2 ** 31 - 3, 10 ** 6])
+def test_max_rows_far_above_the_rows(device, max_rows):
+    """Any bound at or above the entries' rows gives what the tight one gives."""
+    f = Filled(4, 2, 64, [90, 70], 16, seed=2)
+    entries = [(0, 20, 50), (1, 69, 1)]
+    rows = make_rows(entries)
+    loose = KvRows(rows.keep[0].data_ptr(), rows.keep[1].data_ptr(), 2, 51, max_rows, rows.keep[2].data_ptr())
+    k, q = torch.randn(51, 2, 64, generator=f.g, device=DEV), f.q(51)
+    outs = []
+    for r in (rows, loose):
+        o, kr, q2 = torch.empty_like(q), torch.empty_like(k), torch.empty_like(q)
+        f.kv.append(0, q2.data_ptr(), q.data_ptr(), 256, k.data_ptr(), k.data_ptr(), 128, r)
+        f.kv.read(0, kr.data_ptr(), 0, 128, r)
+        f.kv.attend(0, o.data_ptr(), 256, q.data_ptr(), 256, r, 0, f.ws.data_ptr())
+        f.kv.check()
+        outs.append((o, kr, q2))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
