@@ -249,7 +249,8 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(const __grid_cons
 
 template <int R>
 int append_r(const KvAppendParams& p, cudaStream_t s) {
-    const dim3 grid((unsigned)(((int64_t)p.rows.max_rows + AP_ROWS - 1) / AP_ROWS), p.rows.n_seqs);
+    // (a call of no rows too checks its entries)
+    const dim3 grid((unsigned)((std::max<int64_t>(p.rows.max_rows, 1) + AP_ROWS - 1) / AP_ROWS), p.rows.n_seqs);
     auto go = [&](auto kernel) { kernel<<<grid, AP_THREADS, 0, s>>>(p); };
     if (p.qnorm || p.knorm) {
         if (p.rope == BREW_KV_ROPE_HALF) go(kv_append_kernel<R, true, BREW_KV_ROPE_HALF>);
@@ -568,7 +569,7 @@ int brew_kv_append_dev(brew_kv kv, int32_t layer, float* q_out, const float* q, 
         p.knorm = rope->knorm;
         p.eps = rope->eps;
     }
-    if (rows->n_seqs == 0 || rows->n_rows == 0 || rows->max_rows == 0) return BREW_OK;
+    if (rows->n_seqs == 0) return BREW_OK;
     DeviceScope ds;
     if (ds.rc) return ds.rc;
     p.kv = kv_view(kv, layer);
@@ -591,7 +592,7 @@ int brew_kv_read_dev(brew_kv kv, int32_t layer, float* k_out, float* v_out, int6
     if ((k_out && (rc = check_matrix("k_out", k_out, ld, (int64_t)c.n_kv_heads * c.head_size))) ||
         (v_out && (rc = check_matrix("v_out", v_out, ld, (int64_t)c.n_kv_heads * c.head_size))))
         return rc;
-    if (rows->n_seqs == 0 || rows->n_rows == 0 || rows->max_rows == 0) return BREW_OK;
+    if (rows->n_seqs == 0) return BREW_OK;
     DeviceScope ds;
     if (ds.rc) return ds.rc;
     const KvView view = kv_view(kv, layer);
@@ -620,7 +621,7 @@ int brew_kv_attend_dev(brew_kv kv, int32_t layer, float* out, int64_t ldo, const
     BREW_CHECK(std::isfinite(scale), BREW_ERR_INVALID_ARG, "scale %g", (double)scale);
     BREW_CHECK(workspace && ((uintptr_t)workspace & 255) == 0, BREW_ERR_INVALID_ARG,
                "the workspace must be given, on a 256-byte boundary");
-    if (rows->n_seqs == 0 || rows->n_rows == 0 || rows->max_rows == 0) return BREW_OK;
+    if (rows->n_seqs == 0) return BREW_OK;
     DeviceScope ds;
     if (ds.rc) return ds.rc;
     KvAttendParams p = {};

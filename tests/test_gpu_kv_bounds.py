@@ -98,3 +98,35 @@ def test_max_rows_far_above_the_rows(device, max_rows):
         f.kv.check()
         outs.append((o, kr, q2))
     assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+@pytest.mark.parametrize("n_rows,max_rows,start", [(0, 0, [0, 2]), (4, 0, [0, 2]), (0, 5, [0, 1]), (1, 0, None)])
+def test_rows_in_a_call_that_has_none_are_told(device, n_rows, max_rows, start):
+    """Entries with rows where n_rows or max_rows says there are none: skipped and recorded, as any bad entry."""
+    f = Filled(4, 2, 64, [40], 16, seed=3)
+    seq, pos = i32([0]), i32([10])
+    st = i32(start) if start else None
+    x = torch.full((4, 4, 64), 3.0, device=DEV)
+    y = x.clone()
+    rows = KvRows(seq.data_ptr(), pos.data_ptr(), 1, n_rows, max_rows, st.data_ptr() if start else 0)
+    for call in (lambda: f.kv.append(0, y.data_ptr(), x.data_ptr(), 256, x.data_ptr(), x.data_ptr(), 256, rows),
+                 lambda: f.kv.read(0, y.data_ptr(), y.data_ptr(), 256, rows),
+                 lambda: f.kv.attend(0, y.data_ptr(), 256, x.data_ptr(), 256, rows, 0, f.ws.data_ptr())):
+        call()
+        with pytest.raises(N.IllegalStateException):
+            f.kv.check()
+        assert torch.equal(x, y)
+
+
+def test_entries_without_rows_are_no_error(device):
+    f = Filled(4, 2, 64, [40, 7], 16, seed=3)
+    rows = make_rows([(0, 10, 0), (1, 3, 0)])
+    rows.c.max_rows = 0
+    x = torch.full((4, 4, 64), 3.0, device=DEV)
+    y = x.clone()
+    f.kv.append(0, y.data_ptr(), x.data_ptr(), 256, x.data_ptr(), x.data_ptr(), 256, rows)
+    f.kv.read(0, y.data_ptr(), y.data_ptr(), 256, rows)
+    f.kv.attend(0, y.data_ptr(), 256, x.data_ptr(), 256, rows, 0, f.ws.data_ptr())
+    f.kv.check()
+    assert torch.equal(x, y)
+    f.check(f.q(1), [(0, 39, 1)])
