@@ -284,6 +284,11 @@ __global__ void __launch_bounds__(AtShape<R>::THREADS, AtShape<R>::CTAS_PER_SM)
         }
     };
     uint32_t nth = 0;   // tiles this warp has taken
+    // the copies of its next n tiles, which are under way: a CTA that gives up ends behind them
+    auto drain = [&](int n) {
+        for (uint32_t k = nth; k < nth + n; ++k)
+            mbar_wait_bounded(&bars[k % S::STAGES], k / S::STAGES & 1, kv.err, BREW_DEVERR_TIMEOUT_FULL);
+    };
     auto fill = [&](const AtSeg& s) {
         lookup(s, 0);
         for (int k = 0; k < min(s.nt, S::STAGES); ++k) issue(k, nth + k);
@@ -396,10 +401,12 @@ __global__ void __launch_bounds__(AtShape<R>::THREADS, AtShape<R>::CTAS_PER_SM)
         float2 l2 = make_float2(0.0f, 0.0f);
         uint32_t ups = 0;
 
-        for (int k = 0; k < seg.nt; ++k) {
+        int k = 0;
+        for (; k < seg.nt; ++k) {
             const uint32_t slot = nth % S::STAGES;
             if (!mbar_wait_bounded(&bars[slot], nth / S::STAGES & 1, kv.err, BREW_DEVERR_TIMEOUT_FULL)) {
                 s_fail = 1;   // recorded; the CTA stops after this item
+                drain(min(seg.nt - k, S::STAGES));
                 break;
             }
             const uint8_t* tile = ring + slot * S::TILE_BYTES;
@@ -631,10 +638,11 @@ __global__ void __launch_bounds__(AtShape<R>::THREADS, AtShape<R>::CTAS_PER_SM)
 
         // ---- the next item's first tiles, then this one's result
         const int64_t at = u;
+        const bool cut = k < seg.nt;   // this warp gave up
         u = seg.item0 + seg.ub;
         if (tid == 0) s_done = seg;
         __syncwarp();
-        const bool more = u + AT_ITEM < u_end;
+        const bool more = !cut && u + AT_ITEM < u_end;
         if (more) {
             locate(u, seg);
             __syncwarp();
@@ -706,7 +714,10 @@ __global__ void __launch_bounds__(AtShape<R>::THREADS, AtShape<R>::CTAS_PER_SM)
             if (tid == 0) s_ends[at != u_begin] = done;
         }
         __syncthreads();   // the results are read, the next q may be written
-        if (s_fail) return;
+        if (s_fail) {
+            if (more) drain(min(seg.nt, S::STAGES));
+            return;
+        }
         if (!more) break;
     }
 

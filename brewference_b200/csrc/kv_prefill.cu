@@ -347,6 +347,26 @@ __device__ __forceinline__ bool pf_q_store(const KvAttendParams& p, PfRest& sh, 
     return true;
 }
 
+// What a copying or issuing warp (0 .. 3) has under way when it leaves: the last
+// copies have landed, and the last commits (and with them the products) have
+// arrived, before the CTA ends, also where some wait gave up.
+__device__ __noinline__ void pf_drain(PfRest& sh, int warp, int tiles, int items, unsigned int* err) {
+    if (warp == 0) {
+#pragma unroll 1
+        for (int n = max(0, tiles - PF_RAW); n < tiles; ++n) pf_wait_warp(&sh.raw_full[n % PF_RAW], n / PF_RAW & 1, err);
+        return;
+    }
+    const int n = tiles - 1;
+    if (n < 0) return;
+    if (warp == 1) {
+        pf_wait_warp(&sh.k_empty[n & 1], n >> 1 & 1, err);
+        if (items > 0) pf_wait_warp(&sh.q_empty[(items - 1) & 3], (items - 1) >> 2 & 1, err);
+    } else {
+        pf_wait_warp(&sh.o_full[warp - 2], n & 1, err);
+        pf_wait_warp(&sh.p_empty[n & 1], n >> 1 & 1, err);
+    }
+}
+
 // A tile with a scale over 8188, or a NaN: bit 16, whether it is one that some
 // row sees, and a number; below, the positions of group w with a NaN among V's.
 template <int R>
@@ -531,11 +551,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
     // i counts the run's tiles, j its items; a ring's slot and phase follow from them
     if (warp < PF_W_SOFT) {
         regs_dec<PF_REGS_ISSUE>();
+        int i = 0, items = 0;   // tiles that this warp has copied or issued, items that it has issued whole
         if (warp == 0 && len > 0) {
             // ---------------- the run's items, and their copies: a group of 16 positions a lane ----------------
             const int per = 1 << (kv.page_shift - 4);
             PfItem x = sh.item[0];
-            int i = 0;
             bool ok = true;
 #pragma unroll 1
             for (int j = 0; ok; ++j) {
@@ -575,7 +595,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
             constexpr uint32_t idesc = umma_idesc_f16(PF_M, PF_KT);
             const uint64_t kdesc = umma_desc_k(smem_u32(smem + S::K), S::K_PIECE, 128);
             PfItem x;
-            int i = 0;
             bool ok = true;
 #pragma unroll 1
             for (int j = 0; ok && pf_item(sh, j, x, kv.err); ++j) {
@@ -603,8 +622,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
                     __syncwarp();
                 }
                 pf_item_done(sh, j, lane);
-                // the last commit has arrived before the CTA ends
-                if (ok && x.off + x.cnt + PF_ITEM >= len) pf_wait_warp(&sh.q_empty[j & 3], j >> 2 & 1, kv.err);
+                items += ok;
             }
         } else if (warp >= 2 && len > 0) {
             // ---------------- MMA issue: O = p v, a warp for each half of the dims ----------------
@@ -618,12 +636,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
             int j = 0, tiles = 0;
             bool ok = true;
 #pragma unroll 1
-            for (int i = 0; ok; ++i) {
+            for (;; ++i) {
                 if (i == tiles) {
-                    if (!pf_item(sh, j, x, kv.err)) {   // the end: the last commit has arrived before the CTA ends
-                        if (i > 0) pf_wait_warp(&sh.p_empty[(i - 1) & 1], (i - 1) >> 1 & 1, kv.err);
-                        break;
-                    }
+                    if (!pf_item(sh, j, x, kv.err)) break;
                     tiles += x.n;
                     pf_item_done(sh, j++, lane);
                 }
@@ -649,6 +664,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv_prefill_kernel(const __grid_
             }
         }
         __syncwarp();
+        pf_drain(sh, warp, i, items, kv.err);
     } else if (warp < PF_W_SUM) {
         // ---------------- softmax: thread = row, a warpgroup every other tile ----------------
         regs_inc<PF_REGS_SOFT>();
