@@ -1714,7 +1714,6 @@ int brew_model_set_kv_cache(brew_model m, int32_t type) {
     if (rc) return rc;
     std::lock_guard<std::mutex> lk(api_mutex());
     BREW_CUDA(cudaDeviceSynchronize());
-    if ((rc = alloc_unfused(m))) return rc;
     const int B = m->max_batch;
     if (!m->kv_rows && (rc = dalloc(m, &m->kv_rows, (size_t)B + 4))) return rc;
     int32_t ids[MODEL_MAX_BATCH];
@@ -1730,6 +1729,8 @@ int brew_model_set_kv_cache(brew_model m, int32_t type) {
     if ((rc = brew_kv_create(&kc, &kv))) return rc;
     for (int b = 0; b < B && !rc; ++b) rc = brew_kv_reserve(kv, b, c.seq_len, ctx().stream);
     if (!rc && cudaStreamSynchronize(ctx().stream) != cudaSuccess) rc = set_error(BREW_ERR_CUDA, "K/V cache set-up");
+    // last, since it is what changes the forward: a model whose cache cannot be had goes on as it was
+    if (!rc) rc = alloc_unfused(m);
     if (rc) {
         brew_kv_free(kv);
         return rc;

@@ -54,3 +54,26 @@ def test_raise_counters_refusals(device):
     dm = DeviceModel.synthesize(small(C.ARCH_QWEN3), 1)
     assert N.lib().brew_selftest_raise_counters(dm.handle) == N.ERR_INVALID_ARG
     dm.close()
+
+
+def test_a_model_whose_cache_cannot_be_had_goes_on_as_it_was(device):
+    """The device's memory is taken but for a part of what the pool needs."""
+    cfg = small(C.ARCH_LLAMA, seq_len=16384, n_layers=8)
+    dm = DeviceModel.synthesize(cfg, 1, max_batch=16)
+    pool = 2 * 16 * 8 * 16384 * cfg.kv_dim * 18 // 32
+    assert pool > 400 << 20
+    want, kernels = dm.forward([3, 4], [0, 0])[0], dm.step_kernels(3)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    taken = torch.empty(torch.cuda.mem_get_info()[0] - (pool // 2), dtype=torch.uint8, device="cuda")
+    try:
+        with pytest.raises(N.BrewError):
+            dm.set_kv_cache(C.TYPE_Q4_0)
+    finally:
+        del taken
+        torch.cuda.empty_cache()
+    assert np.array_equal(dm.forward([3, 4], [0, 0])[0], want)
+    assert dm.step_kernels(3) == kernels and dm.step_kernels(4) == kernels   # 4: captured only now
+    dm.set_kv_cache(C.TYPE_Q4_0)
+    dm.forward([3, 4], [0, 0])
+    dm.close()
