@@ -462,7 +462,9 @@ class DeviceModel:
 
     def set_kv_cache(self, qtype: int) -> None:
         """The K/V cache: TYPE_F32 (default) or TYPE_Q4_0, the paged 4-bit
-        cache of KvCache (a seventh of the memory; the fp32 one is freed)."""
+        cache of KvCache (a seventh of the memory; the fp32 one is freed
+        once it stands).  One sequence then decodes through separate kernels,
+        more slowly than in the persistent one; long prompts are faster."""
         N.check(N.lib().brew_model_set_kv_cache(self.handle, int(qtype)), "set_kv_cache")
 
     def score(self, tokens, top: int = 0):

@@ -28,11 +28,14 @@
 // tile's K, V and scales are one run per page); the next item's first tiles
 // are under way while an item's warps meet.
 //
-// Bound: instruction issue (unpacking the codes, the split of q, p and p d_V),
-// at 16 warps an SM.  128 sequences of 8192 positions, 28/4 heads of 128: 177
-// us for 608 MB, 3.4 TB/s or 0.52 of a copy's rate; one of 131071, 16/8 heads:
-// 54 us, 2.8 TB/s.  (4 warps a CTA and 3 or 4 CTAs 182 to 184 us; 5 and 3 190;
-// a kernel of its own for the join 4.6 us more on small calls.)
+// Bound: the steps between the copies and the products (unpacking the codes, the
+// split of q, p and p d_V), of which 4 warps a scheduler have too few under way:
+// 54 % of the issue slots are taken, the tensor pipe 32 %, and the largest stalls
+// are an instruction's own latency (1.5 an issue), the math pipe and another
+// warp's turn (1.1 each).  128 sequences of 8192 positions, 28/4 heads of 128: 178
+// us on the device for 608 MB, 3.4 TB/s or 0.52 of a copy's rate; one of 131071,
+// 16/8 heads: 53 us, 2.8 TB/s.  (4 warps a CTA and 3 or 4 CTAs 182 to 184 us; 5
+// and 3 190; a kernel of its own for the join 4.6 us more on small calls.)
 #include <algorithm>
 
 #include "brew_internal.cuh"
@@ -107,7 +110,7 @@ constexpr float AT_PLOG2 = 13.0f;   // p is carried times 2^13, sums and all: p 
 // [2^-8, 1]: they differ little from tile to tile, so that is rare.  The blocks'
 // ups are the nibbles of a register.  (One power for all blocks, from the largest
 // so far, rounded d_V themselves: 60 % off in a block 10^7 below another.  The
-// check costs 1 % of a batch, 186.5 us against 184.7 for 128 sequences of 8192
+// check costs 1.5 % of a batch, 178 us against 176 for 128 sequences of 8192
 // positions; values over 8 cost 14 %, under 0.03 6 %.)
 constexpr int AT_UP_MAX = 14;       // 2^14 is about where fp16 ends
 __device__ __forceinline__ int up_of(uint32_t ups, int b) { return (int)(ups >> 4 * b & 15u); }

@@ -5,7 +5,7 @@
 // of tensor memory.  Keys go by in tiles of 64.  fp32 accuracy comes from
 // fp16 operands in two parts: q and p (hi = fp16(x), lo = fp16(x - hi): 22
 // bits) and the cached values, for which two parts are exact: d (c - 8) has
-// 11 + 4 bits.  Three of the four products are made (lo lo is below 2^-22):
+// 11 + 4 bits (in tiles with values past fp16 the scales under 2^-10 are rounded).  Three of the four products are made (lo lo is below 2^-22):
 //   S = q_hi k_hi + q_hi k_lo + q_lo k_hi,   O = p_hi v_hi + p_hi v_lo + p_lo v_hi
 // so nothing of the blocks' scales is left to the softmax.  q and p are the
 // products' operands in tensor memory (as shared-memory operands they would be
@@ -35,7 +35,7 @@
 //
 // Measured: a tile of 64 keys takes 1.4 us a CTA, where its 48 MMAs of 37
 // cycles take 1.0 (a chunk of 512 rows at 4096 positions, 16/8 heads of 128:
-// 62 us, of which 12 until the first product and 8 from the last to the joined
+// 63 us, of which 12 until the first product and 8 from the last to the joined
 // output).  What bounds it is the other warps' work beside them: 7800 warp
 // instructions a tile at 45% of the issue slots, in loops that have to stay in
 // the instruction cache together (the waits as a dozen instructions each, not
@@ -117,9 +117,8 @@ struct PfRest {
     float2 ml[2][2][PF_M];      // of item j & 1 and a softmax warpgroup: maximum and sum of its tiles
 };
 
-// True in one lane.  In a branch on it the compiler keeps an MMA's operands in
-// uniform registers: 37 cycles from one M128 N64 K16 to the next, 56 in a
-// branch on the lane's number.
+// True in one lane.  In a branch on it 37 cycles go by from one M128 N64 K16 to
+// the next, 56 in a branch on the lane's number.
 __device__ __forceinline__ bool elect_one() {
     uint32_t p = 0;
     asm volatile(

@@ -369,10 +369,14 @@ BREW_API int brew_session_decode(brew_model m, int32_t n_steps, int32_t* out_tok
 BREW_API int brew_model_set_prefill(brew_model m, int32_t mode);
 /* The model's K/V cache.  BREW_TYPE_F32 (the default): dense fp32, as the
  * reference's RunState.  BREW_TYPE_Q4_0: the paged 4-bit cache of brew_kv_*
- * (0.14 of the bytes; the fp32 cache is freed and the session forgotten, and
- * the model stays with it); every forward, prefill (both modes) and session
- * call then goes through brew_kv_append_dev's and brew_kv_attend_dev's
- * kernels in the kernel-graph forward.  K and V are rounded to 4 bits, so
+ * (0.14 of the bytes, pages of seq_len positions for every sequence; the fp32
+ * cache is freed once the other stands and the session forgotten, and the model
+ * stays with it; a context has to fit both for that moment); every forward,
+ * prefill (both modes) and session call then goes through brew_kv_append_dev's
+ * and brew_kv_attend_dev's kernels in the kernel-graph forward of separate
+ * kernels: one sequence decodes more slowly than in the persistent decode
+ * kernel, long prompts and batches faster than before.  When it fails, the
+ * model goes on as it was.  K and V are rounded to 4 bits, so
  * logits differ from the fp32 cache's (brew_session_score shows by how much
  * on a text).  One GPU; head sizes 32, 64, 96, 128, 256; else
  * BREW_ERR_UNSUPPORTED.  No reference counterpart. */
@@ -504,10 +508,10 @@ BREW_API int brew_kv_read_dev(brew_kv kv, int32_t layer, float* k_out, float* v_
  * 0); scale 0 means 1 / sqrt(head_size).  out may not overlap q.  `workspace`:
  * brew_kv_workspace_bytes(kv) device bytes on a 256-byte boundary,
  * zero-filled once before its first use (each call leaves it ready for the
- * next, unless brew_kv_check reports BREW_ERR_TIMEOUT: zero-fill it again then).  Calls and captured
- * graphs that may run at the same time need a workspace each.  Positions that
- * a row does not see may hold anything.  A stored NaN makes the outputs that
- * depend on it NaN (a key's: the row's whole head; a value's: its block of 32
+ * next, unless brew_kv_check reports BREW_ERR_TIMEOUT: zero-fill it again
+ * then).  Calls and captured graphs that may run at the same time need a
+ * workspace each.  Positions that a row does not see may hold anything.  A
+ * stored NaN makes the outputs that depend on it NaN (a key's: the row's whole head; a value's: its block of 32
  * dims or, in entries of many rows, the whole head). */
 BREW_API int64_t brew_kv_workspace_bytes(brew_kv kv);
 BREW_API int brew_kv_attend_dev(brew_kv kv, int32_t layer, float* out, int64_t ldo, const float* q, int64_t ldq,
