@@ -510,11 +510,12 @@ BREW_API int brew_kv_read_dev(brew_kv kv, int32_t layer, float* k_out, float* v_
  * zero-filled once before its first use (each call leaves it ready for the
  * next, unless brew_kv_check reports BREW_ERR_TIMEOUT: zero-fill it again
  * then).  Calls and captured graphs that may run at the same time need a
- * workspace each.  Positions that a row does not see may hold anything (where
- * they hold values past 65504 that a later row of an entry of many rows sees,
- * blocks of values under 0.008 among the same 64 positions keep 2^-20).  A
- * stored NaN makes the outputs that depend on it NaN (a key's: the row's whole head; a value's: its block of 32
- * dims or, in entries of many rows, the whole head). */
+ * workspace each.  Positions that a row does not see may hold anything (only
+ * where they hold values past 65504 that a later row of an entry of many rows
+ * sees are the scales of blocks of values under 0.008, among the same 64
+ * positions, rounded to multiples of 2^-20).  A stored NaN makes the outputs
+ * that depend on it NaN (a key's: the row's whole head; a value's: its block of
+ * 32 dims or, in entries of many rows, the whole head). */
 BREW_API int64_t brew_kv_workspace_bytes(brew_kv kv);
 BREW_API int brew_kv_attend_dev(brew_kv kv, int32_t layer, float* out, int64_t ldo, const float* q, int64_t ldq,
                                 const brew_kv_rows* rows, int32_t window, float scale, void* workspace, void* stream);
